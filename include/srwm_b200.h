@@ -448,6 +448,130 @@ typedef struct srwm_b200_block_args {
 int32_t srwm_b200_block_fits(int32_t rows, int32_t K0, int32_t D, int32_t F, int32_t N);
 int srwm_b200_block_forward(const srwm_b200_block_args* args, void* cuda_stream);
 
+/* ------------------------------------------------------------------------------------
+ * Selective state-space scan and the causal convolution in front of it (no reference kernel corresponds; a third recurrence
+ * beside the two above, with the same uses: sequences with gradients, episode resets, single tokens with the state carried).
+ *   Delta_t = softplus(delta_t + delta_bias),  h_t = exp(Delta_t A) h_{t-1} + (Delta_t u_t) B_t,
+ *   y_t = (C_t . h_t + D u_t) silu(z_t)
+ * for each of D channels with S states.  Rows are [N, L, X] views, innermost contiguous, any other strides (elements), starting
+ * on their elements' alignment; rows whose pieces of four elements are aligned are read four at a time.  B and C are [N, L, G, S]: channel
+ * d reads group d / (D / G).  A [D, S], D, delta_bias [D], states [N, D, S]: dense fp32; A and the states on 16-byte boundaries.
+ * S is 8, 16, 32 or 64 (otherwise ERR_HEAD_DIM); D is a multiple of G.  done [N, L] (bytes, any strides) not zero: the state in
+ * front of step t is zero.  state_out may be state_in.  L == 0 copies the state.
+ * `checkpoints` [N, ceil(L / 8), D, S] (srwm_b200_scan_checkpoint_floats), 16-byte aligned, is written for the backward (NULL: no
+ * backward).  `scratch` (srwm_b200_scan_scratch_bytes / _backward_scratch_bytes, 0: may be NULL) is used during the call.
+ * ---------------------------------------------------------------------------------- */
+typedef struct srwm_b200_rows {     /* [N,L,X] view, innermost contiguous */
+  void*   data;
+  int64_t stride_n, stride_l;             /* elements */
+} srwm_b200_rows;
+typedef struct srwm_b200_scan_args {
+  int32_t N, L, D, S, G;
+  int32_t io_dtype;
+  int32_t softplus;                 /* 0: Delta = delta + delta_bias as given */
+  int32_t reserved;
+  srwm_b200_rows  u, delta;         /* in  [N,L,D] */
+  srwm_b200_rows  z;                /* in  [N,L,D]; data NULL: no gate */
+  srwm_b200_seq   B, C;             /* in  [N,G,L,S] by strides: stride_h is the groups' */
+  const float*    A;
+  const float*    skip;             /* D; NULL: zeros */
+  const float*    delta_bias;       /* NULL: zeros */
+  const float*    state_in;         /* NULL: zeros */
+  const uint8_t*  done;             /* NULL: none */
+  int64_t done_stride_n, done_stride_l;
+  srwm_b200_rows  y;                /* out [N,L,D] (forward) */
+  float*          state_out;        /* NULL: not wanted (forward) */
+  float*          checkpoints;      /* out of the forward, in of the backward */
+  void*           scratch;
+  int64_t         scratch_bytes;
+} srwm_b200_scan_args;
+typedef struct srwm_b200_scan_grads {
+  srwm_b200_rows  dy;               /* in  [N,L,D] */
+  const float*    dstate_out;       /* NULL: zeros */
+  srwm_b200_rows  du, ddelta, dz;   /* out; dz where z is given */
+  srwm_b200_seq   dB, dC;           /* out */
+  float *dA, *dskip, *ddelta_bias;  /* out; the last two may be NULL */
+  float*          dstate_in;        /* NULL: not wanted */
+} srwm_b200_scan_grads;
+int     srwm_b200_scan_forward(const srwm_b200_scan_args* args, void* cuda_stream);
+int     srwm_b200_scan_backward(const srwm_b200_scan_args* args, const srwm_b200_scan_grads* grads, void* cuda_stream);
+int64_t srwm_b200_scan_checkpoint_floats(int32_t N, int32_t L, int32_t D, int32_t S);
+int64_t srwm_b200_scan_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S);
+int64_t srwm_b200_scan_backward_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S, int32_t G);
+
+/* y_t = act(bias + sum_i w[K-1-i] x_{t-i}), act = silu or the identity, K = 2, 3 or 4 taps (otherwise ERR_SHAPE); w [D, K], bias [D] dense
+ * fp32.  state_in / state_out [N, K-1, D] in the rows' type: the last K - 1 inputs before the call and at its end (NULL: zeros / not
+ * wanted); state_out may be state_in where L <= 16.  done as above: no input in front of an episode's start is read behind it.
+ * Backward: dstate_out NULL: zeros; dstate_in, dbias NULL: not wanted; scratch of srwm_b200_conv_scratch_bytes. */
+typedef struct srwm_b200_conv_args {
+  int32_t N, L, D, K;
+  int32_t io_dtype;
+  int32_t silu;
+  srwm_b200_rows  x;                /* in  [N,L,D] */
+  const float*    w;
+  const float*    bias;             /* NULL: zeros */
+  srwm_b200_rows  state_in;
+  const uint8_t*  done;
+  int64_t done_stride_n, done_stride_l;
+  srwm_b200_rows  y, state_out;     /* out (forward) */
+} srwm_b200_conv_args;
+typedef struct srwm_b200_conv_grads {
+  srwm_b200_rows  dy, dstate_out;   /* in  */
+  srwm_b200_rows  dx, dstate_in;    /* out */
+  float *dw, *dbias;
+  void*           scratch;
+  int64_t         scratch_bytes;
+} srwm_b200_conv_grads;
+int     srwm_b200_conv_forward(const srwm_b200_conv_args* args, void* cuda_stream);
+int     srwm_b200_conv_backward(const srwm_b200_conv_args* args, const srwm_b200_conv_grads* grads, void* cuda_stream);
+int64_t srwm_b200_conv_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t K);
+
+/* Root-mean-square norm over rows of D values (D at most 8192), with the residual's addition:
+ *   sum = x + residual (rounded to io_dtype),  y = sum rstd w,  rstd = (mean sum^2 + eps)^-1/2
+ * Rows of x and residual have strides (elements), y and sum are dense.  scale [rows] not NULL: y is e4m3 (one byte a value) and stands for
+ * y scale, scale = max |y| / 448 of the row, at least 2^-126.  residual NULL: none; sum, rstd NULL: not wanted.
+ * Backward: dx (dense; the gradient of x and of the residual) = the norm's + dsum (NULL: none), dw; scratch of
+ * srwm_b200_rms_scratch_bytes; sum are the forward's rows (x where there was no residual). */
+typedef struct srwm_b200_rms_args {
+  int64_t rows;
+  int32_t D, io_dtype;
+  float   eps;
+  int32_t reserved;
+  const void *x, *residual;
+  int64_t x_stride, residual_stride;
+  const float* w;
+  void *y, *sum;
+  float *rstd, *scale;
+} srwm_b200_rms_args;
+typedef struct srwm_b200_rms_grads {
+  int64_t rows;
+  int32_t D, io_dtype;
+  const void *sum, *dy, *dsum;
+  int64_t sum_stride, dy_stride, dsum_stride;
+  const float *w, *rstd;
+  void*   dx;
+  float*  dw;
+  void*   scratch;
+  int64_t scratch_bytes;
+} srwm_b200_rms_grads;
+int     srwm_b200_rms_forward(const srwm_b200_rms_args* args, void* cuda_stream);
+int     srwm_b200_rms_backward(const srwm_b200_rms_grads* args, void* cuda_stream);
+int64_t srwm_b200_rms_scratch_bytes(int64_t rows, int32_t D);
+
+/* Norm of many tensors (dense, io_dtype each; they must not overlap): *norm = sqrt(sum of squares), and with clip each value times
+ * max_norm / (*norm + 1e-6) where that is below 1 (a NaN among the values goes into all).  `tensors` is read on the host during the
+ * call.  scratch of srwm_b200_grads_scratch_bytes, 8-byte aligned. */
+typedef struct srwm_b200_tensor {
+  void*   data;
+  int64_t numel;
+  int32_t io_dtype, reserved;
+} srwm_b200_tensor;
+int     srwm_b200_grads_norm(const srwm_b200_tensor* tensors, int32_t count, float* norm, void* scratch, int64_t scratch_bytes,
+                             void* cuda_stream);
+int     srwm_b200_grads_clip(const srwm_b200_tensor* tensors, int32_t count, float max_norm, float* norm, void* scratch,
+                             int64_t scratch_bytes, void* cuda_stream);
+int64_t srwm_b200_grads_scratch_bytes(const srwm_b200_tensor* tensors, int32_t count);
+
 /* ---- queries (no CUDA call is made by these) ---- */
 int         srwm_b200_abi_version(void);
 int         srwm_b200_head_dim_supported(int32_t E);           /* 1 / 0 */

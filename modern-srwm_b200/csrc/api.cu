@@ -5,9 +5,16 @@
 
 #include "configs.h"
 #include "block.h"
+#include "conv.h"
 #include "gemm.h"
+#include "grads.h"
 #include "launch.h"
 #include "norm.h"
+#include "rms.h"
+#include "scan.h"
+
+#include <new>
+#include <vector>
 
 #ifdef SRWM_DEBUG_CHECKS
 // Status word of the debug build's row checks (common.cuh::bad_rows), one per device.
@@ -907,4 +914,265 @@ extern "C" int srwm_b200_block_forward(const srwm_b200_block_args* a, void* stre
   p.rows = a->rows; p.K0 = a->K0; p.D = a->D; p.F = a->F; p.N = a->N;
   p.eps = a->eps;
   return cuda_result(srwm::block_launch(p, (cudaStream_t)stream));
+}
+
+// ---- selective scan, causal convolution, root-mean-square norm, gradient norm ----
+
+// Rows for the kernels; vec: every piece of four elements (a row has X) starts on its size.
+static srwm::ScanRows scan_rows(const void* data, int64_t sn, int64_t sl, int64_t sg, int X, int es) {
+  srwm::ScanRows r;
+  r.p = (char*)data;
+  r.sn = sn; r.sl = sl; r.sg = sg;
+  r.vec = (uintptr_t)data % (4 * es) == 0 && sn % 4 == 0 && sl % 4 == 0 && sg % 4 == 0 && X % 4 == 0;
+  return r;
+}
+static srwm::ScanRows scan_rows(const srwm_b200_rows& t, int X, int es) { return scan_rows(t.data, t.stride_n, t.stride_l, 0, X, es); }
+static srwm::ScanRows scan_rows(const srwm_b200_seq& t, int X, int es) {
+  return scan_rows(t.data, t.stride_n, t.stride_l, t.stride_h, X, es);
+}
+static bool off(const void* p, int es) { return (uintptr_t)p % es != 0; }
+
+static int scan_sizes(int64_t N, int64_t L, int64_t D, int64_t S, int64_t G) {
+  if (N < 0 || L < 0 || D < 0 || G <= 0 || D % G) return SRWM_B200_ERR_SHAPE;
+  if (!head_dim_ok((int)S)) return SRWM_B200_ERR_HEAD_DIM;
+  const int64_t blocks = (D / G + srwm::SCAN_CH - 1) / srwm::SCAN_CH * G;
+  // one CTA per sequence and 32 channels; four values of dB or dC per thread of the sums' kernel
+  if (blocks * N > 0x7fffffffLL || N * L > 0x7fffffffLL || N * L * G * S / 2 / 256 > 0x7f000000LL) return SRWM_B200_ERR_SHAPE;
+  return 0;
+}
+static int scan_params(const srwm_b200_scan_args* a, srwm::ScanParams* p, bool backward) {
+  if (!a) return SRWM_B200_ERR_NULL;
+  if (int rc = scan_sizes(a->N, a->L, a->D, a->S, a->G)) return rc;
+  if (a->io_dtype != SRWM_B200_F32 && a->io_dtype != SRWM_B200_BF16) return SRWM_B200_ERR_DTYPE;
+  *p = {};
+  p->N = a->N; p->L = a->L; p->D = a->D; p->G = a->G; p->S = a->S;
+  if (a->N == 0 || a->D == 0) return 0;
+  if (!a->A || (a->L > 0 && (!a->u.data || !a->delta.data || !a->B.data || !a->C.data))) return SRWM_B200_ERR_NULL;
+  const int es = esize(a->io_dtype);
+  for (const void* d : {(const void*)a->A, (const void*)a->state_in, (const void*)a->state_out, (const void*)a->checkpoints})
+    if (off(d, 16)) return SRWM_B200_ERR_ALIGN;
+  for (const void* d : {(const void*)a->skip, (const void*)a->delta_bias})
+    if (off(d, 4)) return SRWM_B200_ERR_ALIGN;
+  for (const void* d : {a->u.data, a->delta.data, a->z.data, a->y.data, a->B.data, a->C.data})
+    if (off(d, es)) return SRWM_B200_ERR_ALIGN;
+  const int Dg = a->D / a->G;
+  p->bf16 = a->io_dtype == SRWM_B200_BF16;
+  p->softplus = a->softplus != 0;
+  p->u = scan_rows(a->u, Dg, es); p->delta = scan_rows(a->delta, Dg, es);
+  p->z = scan_rows(a->z, Dg, es); p->y = scan_rows(a->y, Dg, es);
+  p->B = scan_rows(a->B, a->S, es); p->C = scan_rows(a->C, a->S, es);
+  p->A = a->A; p->skip = a->skip; p->bias = a->delta_bias; p->h0 = a->state_in; p->hT = a->state_out;
+  p->done = a->done; p->done_n = a->done_stride_n; p->done_l = a->done_stride_l;
+  p->ckpt = a->checkpoints;
+  p->nseg = backward ? srwm::scan_bwd_segments(a->N, a->L, a->D, srwm::common_sms()) : srwm::scan_segments(a->N, a->L, a->D, srwm::common_sms());
+  const int per = (a->L + p->nseg - 1) / p->nseg;
+  p->seglen = (per + srwm::SCAN_TILE - 1) / srwm::SCAN_TILE * srwm::SCAN_TILE;
+  if (p->seglen > 0) p->nseg = (a->L + p->seglen - 1) / p->seglen;      // (rounded up, fewer pieces may do)
+  if (p->nseg < 1) p->nseg = 1;
+  return 0;
+}
+// As scan_params sets them, for the questions about sizes
+static srwm::ScanParams scan_shape(int32_t N, int32_t L, int32_t D, int32_t S, int32_t G, bool backward) {
+  srwm_b200_scan_args a = {};
+  static const float dummy[4] __attribute__((aligned(16))) = {};
+  a.N = N; a.L = L; a.D = D; a.S = S; a.G = G;
+  a.A = dummy;
+  a.u.data = a.delta.data = a.B.data = a.C.data = (void*)dummy;
+  srwm::ScanParams p = {};
+  if (scan_params(&a, &p, backward) != 0) p = {};
+  return p;
+}
+
+extern "C" int64_t srwm_b200_scan_checkpoint_floats(int32_t N, int32_t L, int32_t D, int32_t S) {
+  return N <= 0 || L <= 0 || D <= 0 || S <= 0 ? 0 : (int64_t)N * ((L + srwm::SCAN_CKPT - 1) / srwm::SCAN_CKPT) * D * S;
+}
+extern "C" int64_t srwm_b200_scan_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S) {
+  return 4 * srwm::scan_fwd_scratch(scan_shape(N, L, D, S, 1, false));
+}
+extern "C" int64_t srwm_b200_scan_backward_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S, int32_t G) {
+  srwm::ScanParams p = scan_shape(N, L, D, S, G, true);
+  return p.G == 0 ? 0 : 4 * srwm::scan_bwd_scratch(p, nullptr);
+}
+
+extern "C" int srwm_b200_scan_forward(const srwm_b200_scan_args* a, void* stream) {
+  srwm::ScanParams p;
+  if (int rc = scan_params(a, &p, false)) return rc;
+  if (a->N == 0 || a->D == 0) return 0;
+  if (a->L > 0 && !a->y.data) return SRWM_B200_ERR_NULL;
+  const int64_t need = 4 * srwm::scan_fwd_scratch(p);
+  if (need > 0 && (!a->scratch || a->scratch_bytes < need)) return SRWM_B200_ERR_NULL;
+  if (off(a->scratch, 16)) return SRWM_B200_ERR_ALIGN;
+  p.carry = (float*)a->scratch;
+  return cuda_result(srwm::scan_forward(p, (cudaStream_t)stream));
+}
+
+extern "C" int srwm_b200_scan_backward(const srwm_b200_scan_args* a, const srwm_b200_scan_grads* g, void* stream) {
+  srwm::ScanParams p;
+  if (!g) return SRWM_B200_ERR_NULL;
+  if (int rc = scan_params(a, &p, true)) return rc;
+  if (a->N == 0 || a->D == 0) return 0;
+  if (a->L == 0) return SRWM_B200_ERR_SHAPE;
+  if (!a->checkpoints || !g->dy.data || !g->du.data || !g->ddelta.data || (a->z.data && !g->dz.data) || !g->dB.data || !g->dC.data || !g->dA)
+    return SRWM_B200_ERR_NULL;
+  const int es = esize(a->io_dtype), Dg = a->D / a->G;
+  for (const void* d : {g->dy.data, g->du.data, g->ddelta.data, g->dz.data, g->dB.data, g->dC.data})
+    if (off(d, es)) return SRWM_B200_ERR_ALIGN;
+  for (const void* d : {(const void*)g->dstate_out, (const void*)g->dstate_in, (const void*)a->scratch})
+    if (off(d, 16)) return SRWM_B200_ERR_ALIGN;
+  for (const void* d : {(const void*)g->dA, (const void*)g->dskip, (const void*)g->ddelta_bias})
+    if (off(d, 4)) return SRWM_B200_ERR_ALIGN;
+  const int64_t need = 4 * srwm::scan_bwd_scratch(p, nullptr);
+  if (!a->scratch || a->scratch_bytes < need) return SRWM_B200_ERR_NULL;
+  srwm::scan_bwd_scratch(p, (float*)a->scratch);
+  p.dy = scan_rows(g->dy, Dg, es); p.du = scan_rows(g->du, Dg, es);
+  p.ddelta = scan_rows(g->ddelta, Dg, es); p.dz = scan_rows(g->dz, Dg, es);
+  p.dB = scan_rows(g->dB, a->S, es); p.dC = scan_rows(g->dC, a->S, es);
+  p.dhT = g->dstate_out; p.dh0 = g->dstate_in; p.dA = g->dA; p.dskip = g->dskip; p.dbias = g->ddelta_bias;
+  return cuda_result(srwm::scan_backward(p, (cudaStream_t)stream));
+}
+
+static int conv_params(const srwm_b200_conv_args* a, srwm::ConvParams* p) {
+  if (!a) return SRWM_B200_ERR_NULL;
+  if (a->N < 0 || a->L < 0 || a->D < 0 || a->K < 2 || a->K > 4) return SRWM_B200_ERR_SHAPE;
+  if (a->io_dtype != SRWM_B200_F32 && a->io_dtype != SRWM_B200_BF16) return SRWM_B200_ERR_DTYPE;
+  const int64_t chunks = a->L == 0 ? 1 : (a->L + srwm::CONV_CHUNK - 1) / srwm::CONV_CHUNK;
+  if ((a->D + 3ll) / 4 * chunks / 128 * a->N > 0x7f000000LL) return SRWM_B200_ERR_SHAPE;
+  *p = {};
+  p->N = a->N; p->L = a->L; p->D = a->D; p->K = a->K;
+  if (a->N == 0 || a->D == 0) return 0;
+  if (!a->w || (a->L > 0 && !a->x.data)) return SRWM_B200_ERR_NULL;
+  const int es = esize(a->io_dtype);
+  for (const void* d : {a->x.data, a->y.data, a->state_in.data, a->state_out.data})
+    if (off(d, es)) return SRWM_B200_ERR_ALIGN;
+  for (const void* d : {(const void*)a->w, (const void*)a->bias})
+    if (off(d, 4)) return SRWM_B200_ERR_ALIGN;
+  p->bf16 = a->io_dtype == SRWM_B200_BF16;
+  p->silu = a->silu != 0;
+  p->x = scan_rows(a->x, a->D, es); p->y = scan_rows(a->y, a->D, es);
+  p->s0 = scan_rows(a->state_in, a->D, es); p->sT = scan_rows(a->state_out, a->D, es);
+  p->w = a->w; p->bias = a->bias;
+  p->done = a->done; p->done_n = a->done_stride_n; p->done_l = a->done_stride_l;
+  return 0;
+}
+extern "C" int64_t srwm_b200_conv_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t K) {
+  if (N <= 0 || L <= 0 || D <= 0 || K < 2 || K > 4) return 0;
+  srwm::ConvParams p = {};
+  p.N = N; p.L = L; p.D = D; p.K = K;
+  return 4ll * srwm::conv_parts(p) * D * (K + 1);
+}
+extern "C" int srwm_b200_conv_forward(const srwm_b200_conv_args* a, void* stream) {
+  srwm::ConvParams p;
+  if (int rc = conv_params(a, &p)) return rc;
+  if (a->N == 0 || a->D == 0) return 0;
+  if (a->L > 0 && !a->y.data) return SRWM_B200_ERR_NULL;
+  // (a thread reads its window before it writes the state; with several chunks of steps another one might not have yet)
+  if (a->L > srwm::CONV_CHUNK && a->state_out.data && a->state_out.data == a->state_in.data) return SRWM_B200_ERR_UNSUPPORTED;
+  return cuda_result(srwm::conv_forward(p, (cudaStream_t)stream));
+}
+extern "C" int srwm_b200_conv_backward(const srwm_b200_conv_args* a, const srwm_b200_conv_grads* g, void* stream) {
+  srwm::ConvParams p;
+  if (!g) return SRWM_B200_ERR_NULL;
+  if (int rc = conv_params(a, &p)) return rc;
+  if (a->N == 0 || a->D == 0) return 0;
+  if (a->L == 0) return SRWM_B200_ERR_SHAPE;
+  if (!g->dy.data || !g->dx.data || !g->dw || !g->scratch || g->scratch_bytes < srwm_b200_conv_scratch_bytes(a->N, a->L, a->D, a->K))
+    return SRWM_B200_ERR_NULL;
+  const int es = esize(a->io_dtype);
+  for (const void* d : {g->dy.data, g->dx.data, g->dstate_in.data, g->dstate_out.data})
+    if (off(d, es)) return SRWM_B200_ERR_ALIGN;
+  for (const void* d : {(const void*)g->dw, (const void*)g->dbias, (const void*)g->scratch})
+    if (off(d, 4)) return SRWM_B200_ERR_ALIGN;
+  p.dy = scan_rows(g->dy, a->D, es); p.dx = scan_rows(g->dx, a->D, es);
+  p.dsT = scan_rows(g->dstate_out, a->D, es); p.ds0 = scan_rows(g->dstate_in, a->D, es);
+  p.dw = g->dw; p.dbias = g->dbias; p.part = (float*)g->scratch;
+  return cuda_result(srwm::conv_backward(p, (cudaStream_t)stream));
+}
+
+static int rms_check(int64_t rows, int32_t D, int32_t dtype) {
+  if (rows < 0 || D <= 0 || D > srwm::RMS_MAX_D) return SRWM_B200_ERR_SHAPE;
+  return dtype != SRWM_B200_F32 && dtype != SRWM_B200_BF16 ? SRWM_B200_ERR_DTYPE : 0;
+}
+extern "C" int srwm_b200_rms_forward(const srwm_b200_rms_args* a, void* stream) {
+  if (!a) return SRWM_B200_ERR_NULL;
+  if (int rc = rms_check(a->rows, a->D, a->io_dtype)) return rc;
+  if (a->rows == 0) return 0;
+  if (!a->x || !a->w || !a->y) return SRWM_B200_ERR_NULL;
+  const int es = esize(a->io_dtype);
+  if (off(a->x, es) || off(a->residual, es) || off(a->sum, es) || off(a->w, 4) || off(a->rstd, 4) || off(a->scale, 4) ||
+      (!a->scale && off(a->y, es)))
+    return SRWM_B200_ERR_ALIGN;
+  srwm::RmsParams p = {};
+  p.x = a->x; p.res = a->residual; p.x_row = a->x_stride; p.res_row = a->residual_stride;
+  p.w = a->w; p.y = a->y; p.sum = a->sum; p.rstd = a->rstd; p.scale = a->scale;
+  p.rows = a->rows; p.D = a->D; p.bf16 = a->io_dtype == SRWM_B200_BF16; p.fp8 = a->scale != nullptr; p.eps = a->eps;
+  return cuda_result(srwm::rms_forward(p, (cudaStream_t)stream));
+}
+extern "C" int64_t srwm_b200_rms_scratch_bytes(int64_t rows, int32_t D) {
+  return rows <= 0 || D <= 0 ? 0 : 4ll * srwm::rms_blocks(rows, D) * D;
+}
+extern "C" int srwm_b200_rms_backward(const srwm_b200_rms_grads* a, void* stream) {
+  if (!a) return SRWM_B200_ERR_NULL;
+  if (int rc = rms_check(a->rows, a->D, a->io_dtype)) return rc;
+  if (a->rows == 0) return 0;
+  if (!a->sum || !a->dy || !a->w || !a->rstd || !a->dx || !a->dw || !a->scratch ||
+      a->scratch_bytes < srwm_b200_rms_scratch_bytes(a->rows, a->D))
+    return SRWM_B200_ERR_NULL;
+  const int es = esize(a->io_dtype);
+  for (const void* d : {a->sum, a->dy, a->dsum, (const void*)a->dx})
+    if (off(d, es)) return SRWM_B200_ERR_ALIGN;
+  for (const void* d : {(const void*)a->w, (const void*)a->rstd, (const void*)a->dw, (const void*)a->scratch})
+    if (off(d, 4)) return SRWM_B200_ERR_ALIGN;
+  srwm::RmsParams p = {};
+  p.sum = const_cast<void*>(a->sum); p.sum_row = a->sum_stride;
+  p.dy = a->dy; p.dy_row = a->dy_stride; p.dsum = a->dsum; p.dsum_row = a->dsum_stride;
+  p.w = a->w; p.rstd = const_cast<float*>(a->rstd); p.y = a->dx; p.dw = a->dw; p.part = (float*)a->scratch;
+  p.rows = a->rows; p.D = a->D; p.bf16 = a->io_dtype == SRWM_B200_BF16;
+  return cuda_result(srwm::rms_backward(p, (cudaStream_t)stream));
+}
+
+// The caller's list as the kernels take it, without empty tensors
+static int grad_list(const srwm_b200_tensor* t, int32_t count, std::vector<srwm::GradTensor>* out) {
+  if (count < 0) return SRWM_B200_ERR_SHAPE;
+  if (count > 0 && !t) return SRWM_B200_ERR_NULL;
+  try {
+    out->reserve((size_t)count);
+  } catch (const std::bad_alloc&) {
+    return SRWM_B200_ERR_TOO_LARGE;
+  }
+  int64_t chunks = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    if (t[i].numel < 0) return SRWM_B200_ERR_SHAPE;
+    if (t[i].io_dtype != SRWM_B200_F32 && t[i].io_dtype != SRWM_B200_BF16) return SRWM_B200_ERR_DTYPE;
+    if (t[i].numel == 0) continue;
+    if (!t[i].data) return SRWM_B200_ERR_NULL;
+    if (off(t[i].data, esize(t[i].io_dtype))) return SRWM_B200_ERR_ALIGN;
+    chunks += (t[i].numel - 1) / srwm::GRADS_CHUNK + 1;
+    if (chunks > 0x7f000000LL) return SRWM_B200_ERR_SHAPE;
+    out->push_back({t[i].data, (long long)t[i].numel, t[i].io_dtype == SRWM_B200_BF16});
+  }
+  return 0;
+}
+extern "C" int64_t srwm_b200_grads_scratch_bytes(const srwm_b200_tensor* t, int32_t count) {
+  std::vector<srwm::GradTensor> v;
+  return grad_list(t, count, &v) != 0 ? 0 : 8ll * srwm::grads_parts(v.data(), (int)v.size());
+}
+static int grads_call(const srwm_b200_tensor* t, int32_t count, const float* max_norm, float* norm, void* scratch, int64_t bytes,
+                      void* stream) {
+  std::vector<srwm::GradTensor> v;
+  if (int rc = grad_list(t, count, &v)) return rc;
+  if (!norm || !scratch || bytes < 8ll * srwm::grads_parts(v.data(), (int)v.size())) return SRWM_B200_ERR_NULL;
+  if (off(norm, 4) || off(scratch, 8)) return SRWM_B200_ERR_ALIGN;
+  const cudaStream_t s = (cudaStream_t)stream;
+  const cudaError_t e = srwm::grads_norm(v.data(), (int)v.size(), (double*)scratch, max_norm ? nullptr : norm, s);
+  if (e != cudaSuccess || !max_norm) return cuda_result(e);
+  return cuda_result(srwm::grads_clip(v.data(), (int)v.size(), (const double*)scratch, *max_norm, norm, s));
+}
+extern "C" int srwm_b200_grads_norm(const srwm_b200_tensor* tensors, int32_t count, float* norm, void* scratch, int64_t scratch_bytes,
+                                    void* stream) {
+  return grads_call(tensors, count, nullptr, norm, scratch, scratch_bytes, stream);
+}
+extern "C" int srwm_b200_grads_clip(const srwm_b200_tensor* tensors, int32_t count, float max_norm, float* norm, void* scratch,
+                                    int64_t scratch_bytes, void* stream) {
+  if (!(max_norm >= 0.f)) return SRWM_B200_ERR_SHAPE;
+  return grads_call(tensors, count, &max_norm, norm, scratch, scratch_bytes, stream);
 }

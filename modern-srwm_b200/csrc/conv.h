@@ -1,0 +1,27 @@
+// Causal convolution of a few steps along time (conv.cu).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "scan.h"
+
+namespace srwm {
+
+constexpr int CONV_CHUNK = 16;     // steps of a thread at most
+
+struct ConvParams {
+  int N, L, D, K;
+  int bf16, silu;
+  ScanRows x, y, s0, sT;           // [N, L, D]; the states [N, K-1, D], NULL: zeros / not wanted
+  const float *w, *bias;           // [D, K], [D] or NULL
+  const uint8_t* done;
+  long long done_n, done_l;
+  // backward
+  ScanRows dy, dx, dsT, ds0;
+  float *dw, *dbias, *part;
+};
+int conv_parts(const ConvParams& p);          // the backward's partial sums [conv_parts][D][K + 1]
+cudaError_t conv_forward(const ConvParams& p, cudaStream_t s);
+cudaError_t conv_backward(const ConvParams& p, cudaStream_t s);
+
+}  // namespace srwm

@@ -1,5 +1,6 @@
 // Python module srwm_b200._host: see host_common.h.
 #include "host_layers.h"
+#include "host_ops.h"
 
 namespace {
 using namespace host;
@@ -221,6 +222,89 @@ PyObject* block_tail_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// (u, delta, A, B, C, D, z, delta_bias, state, done, softplus, inplace) -> y, state
+PyObject* scan_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 12)) return nullptr;
+  Tensor t[10];
+  if (forward_ad() || !take(args, 0, 5, t) || !take(args, 5, 5, t + 5, true)) return declined();
+  const ScanIn s = {t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], PyObject_IsTrue(args[10]) != 0};
+  const bool inplace = PyObject_IsTrue(args[11]);
+  const bool grad = wants_grad({&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8]});
+  if (!scan_ok(s) || (inplace && (grad || !s.state.defined()))) return declined();
+  variable_list r;
+  {
+    NoGil nogil;
+    if (grad) r = Scan::apply(s.u, s.delta, s.A, s.B, s.C, opt(s.D), opt(s.z), opt(s.bias), opt(s.state), opt(s.done), s.softplus);
+    else r = scan_forward(s, inplace, nullptr);
+  }
+  return wrap(r);
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, weight, bias, state, done, silu, inplace) -> y, state
+PyObject* conv_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 7)) return nullptr;
+  Tensor t[5];
+  if (forward_ad() || !take(args, 0, 2, t) || !take(args, 2, 3, t + 2, true)) return declined();
+  const ConvIn s = {t[0], t[1], t[2], t[3], t[4], PyObject_IsTrue(args[5]) != 0};
+  const bool inplace = PyObject_IsTrue(args[6]), grad = wants_grad({&t[0], &t[1], &t[2], &t[3]});
+  if (!conv_ok(s) || (inplace && (grad || !s.state.defined()))) return declined();
+  variable_list r;
+  {
+    NoGil nogil;
+    if (grad) r = Conv::apply(s.x, s.w, opt(s.bias), opt(s.state), opt(s.done), s.silu);
+    else r = conv_forward(s, inplace);
+  }
+  return wrap(r);
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, weight, residual or None, eps, fp8) -> y[, scale][, x + residual]
+PyObject* rms_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 5)) return nullptr;
+  Tensor t[2], res;
+  const double eps = PyFloat_AsDouble(args[3]);
+  if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+  const bool fp8 = PyObject_IsTrue(args[4]);
+  if (forward_ad() || !take(args, 0, 2, t) || !take(args, 2, 1, &res, true) || !rms_ok(t[0], t[1], res)) return declined();
+  const bool grad = wants_grad({&t[0], &t[1], &res});
+  if (grad && fp8) return declined();
+  variable_list r;
+  {
+    NoGil nogil;
+    if (grad) r = Rms::apply(t[0], t[1], opt(res), eps);
+    else r = rms_forward(t[0], t[1], res, eps, fp8, nullptr);
+  }
+  return r.size() == 1 ? THPVariable_Wrap(r[0]) : wrap(r);
+  END_HANDLE_TH_ERRORS
+}
+
+// (list of tensors, max_norm or a negative number) -> norm; with a max_norm the tensors are scaled in place
+PyObject* grads_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 2)) return nullptr;
+  const double max_norm = PyFloat_AsDouble(args[1]);
+  if (max_norm == -1.0 && PyErr_Occurred()) return nullptr;
+  if (!PyList_Check(args[0])) return declined();
+  std::vector<Tensor> ts((size_t)PyList_GET_SIZE(args[0]));
+  for (size_t i = 0; i < ts.size(); ++i) {
+    PyObject* o = PyList_GET_ITEM(args[0], (Py_ssize_t)i);
+    if (!plain(o)) return declined();
+    ts[i] = THPVariable_Unpack(o);
+  }
+  if (ts.empty() || !grads_ok(ts)) return declined();
+  Tensor norm;
+  {
+    NoGil nogil;
+    norm = grads_norm(ts, max_norm);
+  }
+  return THPVariable_Wrap(norm);
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
                          {"self_ref_v0", FAST(self_ref)},
@@ -233,6 +317,10 @@ PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
                          {"ff_step", FAST(ff_step_py)},
                          {"layer_norm", FAST(norm_py)},
                          {"block_tail", FAST(block_tail_py)},
+                         {"selective_scan", FAST(scan_py)},
+                         {"causal_conv", FAST(conv_py)},
+                         {"rms_norm", FAST(rms_py)},
+                         {"grads_norm", FAST(grads_py)},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 }  // namespace

@@ -45,7 +45,21 @@ using torch::autograd::variable_list;
   X(srwm_b200_norm_scratch_bytes)                                                                     \
   X(srwm_b200_norm_backward)                                                                          \
   X(srwm_b200_block_fits)                                                                             \
-  X(srwm_b200_block_forward)
+  X(srwm_b200_block_forward)                                                                          \
+  X(srwm_b200_scan_forward)                                                                           \
+  X(srwm_b200_scan_backward)                                                                          \
+  X(srwm_b200_scan_checkpoint_floats)                                                                 \
+  X(srwm_b200_scan_scratch_bytes)                                                                     \
+  X(srwm_b200_scan_backward_scratch_bytes)                                                            \
+  X(srwm_b200_conv_forward)                                                                           \
+  X(srwm_b200_conv_backward)                                                                          \
+  X(srwm_b200_conv_scratch_bytes)                                                                     \
+  X(srwm_b200_rms_forward)                                                                            \
+  X(srwm_b200_rms_backward)                                                                           \
+  X(srwm_b200_rms_scratch_bytes)                                                                      \
+  X(srwm_b200_grads_norm)                                                                             \
+  X(srwm_b200_grads_clip)                                                                             \
+  X(srwm_b200_grads_scratch_bytes)
 
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;

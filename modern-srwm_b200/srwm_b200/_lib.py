@@ -108,6 +108,50 @@ class BlockArgs(C.Structure):
                [(n, C.c_int32) for n in ("rows", "K0", "D", "F", "N")] + [("eps", C.c_float)]
 
 
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride_n", C.c_int64), ("stride_l", C.c_int64)]
+
+
+class ScanArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("N", "L", "D", "S", "G", "io_dtype", "softplus", "reserved")] + \
+               [("u", Rows), ("delta", Rows), ("z", Rows), ("B", Seq), ("C", Seq)] + \
+               [(n, C.c_void_p) for n in ("A", "skip", "delta_bias", "state_in", "done")] + \
+               [("done_stride_n", C.c_int64), ("done_stride_l", C.c_int64), ("y", Rows), ("state_out", C.c_void_p),
+                ("checkpoints", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_int64)]
+
+
+class ScanGrads(C.Structure):
+    _fields_ = [("dy", Rows), ("dstate_out", C.c_void_p), ("du", Rows), ("ddelta", Rows), ("dz", Rows), ("dB", Seq), ("dC", Seq)] + \
+               [(n, C.c_void_p) for n in ("dA", "dskip", "ddelta_bias", "dstate_in")]
+
+
+class ConvArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("N", "L", "D", "K", "io_dtype", "silu")] + \
+               [("x", Rows), ("w", C.c_void_p), ("bias", C.c_void_p), ("state_in", Rows), ("done", C.c_void_p),
+                ("done_stride_n", C.c_int64), ("done_stride_l", C.c_int64), ("y", Rows), ("state_out", Rows)]
+
+
+class ConvGrads(C.Structure):
+    _fields_ = [("dy", Rows), ("dstate_out", Rows), ("dx", Rows), ("dstate_in", Rows), ("dw", C.c_void_p), ("dbias", C.c_void_p),
+                ("scratch", C.c_void_p), ("scratch_bytes", C.c_int64)]
+
+
+class RmsArgs(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("D", C.c_int32), ("io_dtype", C.c_int32), ("eps", C.c_float), ("reserved", C.c_int32),
+                ("x", C.c_void_p), ("residual", C.c_void_p), ("x_stride", C.c_int64), ("residual_stride", C.c_int64)] + \
+               [(n, C.c_void_p) for n in ("w", "y", "sum", "rstd", "scale")]
+
+
+class RmsGrads(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("D", C.c_int32), ("io_dtype", C.c_int32), ("sum", C.c_void_p), ("dy", C.c_void_p),
+                ("dsum", C.c_void_p), ("sum_stride", C.c_int64), ("dy_stride", C.c_int64), ("dsum_stride", C.c_int64)] + \
+               [(n, C.c_void_p) for n in ("w", "rstd", "dx", "dw", "scratch")] + [("scratch_bytes", C.c_int64)]
+
+
+class TensorDesc(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("numel", C.c_int64), ("io_dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
 class DeltaPackedFwdArgs(C.Structure):
     _fields_ = [("N", C.c_int32), ("H", C.c_int32), ("L", C.c_int32), ("E", C.c_int32),
                 ("io_dtype", C.c_int32), ("flags", C.c_uint32), ("variant", C.c_int32),
@@ -154,6 +198,20 @@ SYMBOLS = {
     "srwm_b200_norm_backward": (C.c_int, [C.c_void_p] * 8 + [C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     "srwm_b200_block_fits": (C.c_int32, [C.c_int32] * 5),
     "srwm_b200_block_forward": (C.c_int, [C.POINTER(BlockArgs), C.c_void_p]),
+    "srwm_b200_scan_forward": (C.c_int, [C.POINTER(ScanArgs), C.c_void_p]),
+    "srwm_b200_scan_backward": (C.c_int, [C.POINTER(ScanArgs), C.POINTER(ScanGrads), C.c_void_p]),
+    "srwm_b200_scan_checkpoint_floats": (C.c_int64, [C.c_int32] * 4),
+    "srwm_b200_scan_scratch_bytes": (C.c_int64, [C.c_int32] * 4),
+    "srwm_b200_scan_backward_scratch_bytes": (C.c_int64, [C.c_int32] * 5),
+    "srwm_b200_conv_forward": (C.c_int, [C.POINTER(ConvArgs), C.c_void_p]),
+    "srwm_b200_conv_backward": (C.c_int, [C.POINTER(ConvArgs), C.POINTER(ConvGrads), C.c_void_p]),
+    "srwm_b200_conv_scratch_bytes": (C.c_int64, [C.c_int32] * 4),
+    "srwm_b200_rms_forward": (C.c_int, [C.POINTER(RmsArgs), C.c_void_p]),
+    "srwm_b200_rms_backward": (C.c_int, [C.POINTER(RmsGrads), C.c_void_p]),
+    "srwm_b200_rms_scratch_bytes": (C.c_int64, [C.c_int64, C.c_int32]),
+    "srwm_b200_grads_norm": (C.c_int, [C.POINTER(TensorDesc), C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "srwm_b200_grads_clip": (C.c_int, [C.POINTER(TensorDesc), C.c_int32, C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "srwm_b200_grads_scratch_bytes": (C.c_int64, [C.POINTER(TensorDesc), C.c_int32]),
     "srwm_b200_debug_status": (C.c_int, [C.POINTER(C.c_uint64)]),
     "srwm_b200_debug_selftest": (C.c_int, [C.c_void_p]),
     "srwm_b200_debug_gemm_tries": (C.c_int, [C.c_int32]),

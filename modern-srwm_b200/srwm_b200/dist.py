@@ -67,6 +67,16 @@ class GradBucket:
         self.work = dist.all_reduce(self.flat, op=dist.ReduceOp.SUM, group=group, async_op=async_op)
         return self.work
 
+    def clip_(self, max_norm):
+        """The bucket times ``max_norm / (norm + 1e-6)`` where that is below 1, in place (after the all-reduce: every rank has the
+        same values then).  Returns the 2-norm before, on the device."""
+        if self.flat.device.type == "cuda":
+            from .grad_ops import clip_tensors_
+            return clip_tensors_([self.flat], max_norm)
+        norm = self.flat.norm()
+        self.flat.mul_(torch.clamp(max_norm / (norm + 1e-6), max=1.0))
+        return norm
+
     def wait(self):
         if self.work is not None:
             self.work.wait()
