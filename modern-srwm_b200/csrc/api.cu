@@ -918,17 +918,16 @@ extern "C" int srwm_b200_block_forward(const srwm_b200_block_args* a, void* stre
 
 // ---- selective scan, causal convolution, root-mean-square norm, gradient norm ----
 
-// Rows for the kernels; vec: every piece of four elements (a row has X) starts on its size.
-static srwm::ScanRows scan_rows(const void* data, int64_t sn, int64_t sl, int64_t sg, int X, int es) {
-  srwm::ScanRows r;
-  r.p = (char*)data;
-  r.sn = sn; r.sl = sl; r.sg = sg;
-  r.vec = (uintptr_t)data % (4 * es) == 0 && sn % 4 == 0 && sl % 4 == 0 && sg % 4 == 0 && X % 4 == 0;
-  return r;
+// Rows for the kernels; *vec stays set while every piece of four elements (a row has X) starts on its size.
+static srwm::ScanRows scan_rows(const void* data, int64_t sn, int64_t sl, int64_t sg, int X, int es, int* vec) {
+  if (data && ((uintptr_t)data % (4 * es) || sn % 4 || sl % 4 || sg % 4 || X % 4)) *vec = 0;
+  return {(char*)data, sn, sl, sg};
 }
-static srwm::ScanRows scan_rows(const srwm_b200_rows& t, int X, int es) { return scan_rows(t.data, t.stride_n, t.stride_l, 0, X, es); }
-static srwm::ScanRows scan_rows(const srwm_b200_seq& t, int X, int es) {
-  return scan_rows(t.data, t.stride_n, t.stride_l, t.stride_h, X, es);
+static srwm::ScanRows scan_rows(const srwm_b200_rows& t, int X, int es, int* vec) {
+  return scan_rows(t.data, t.stride_n, t.stride_l, 0, X, es, vec);
+}
+static srwm::ScanRows scan_rows(const srwm_b200_seq& t, int X, int es, int* vec) {
+  return scan_rows(t.data, t.stride_n, t.stride_l, t.stride_h, X, es, vec);
 }
 static bool off(const void* p, int es) { return (uintptr_t)p % es != 0; }
 
@@ -958,9 +957,10 @@ static int scan_params(const srwm_b200_scan_args* a, srwm::ScanParams* p, bool b
   const int Dg = a->D / a->G;
   p->bf16 = a->io_dtype == SRWM_B200_BF16;
   p->softplus = a->softplus != 0;
-  p->u = scan_rows(a->u, Dg, es); p->delta = scan_rows(a->delta, Dg, es);
-  p->z = scan_rows(a->z, Dg, es); p->y = scan_rows(a->y, Dg, es);
-  p->B = scan_rows(a->B, a->S, es); p->C = scan_rows(a->C, a->S, es);
+  p->vec = 1;
+  p->u = scan_rows(a->u, Dg, es, &p->vec); p->delta = scan_rows(a->delta, Dg, es, &p->vec);
+  p->z = scan_rows(a->z, Dg, es, &p->vec); p->y = scan_rows(a->y, Dg, es, &p->vec);
+  p->B = scan_rows(a->B, a->S, es, &p->vec); p->C = scan_rows(a->C, a->S, es, &p->vec);
   p->A = a->A; p->skip = a->skip; p->bias = a->delta_bias; p->h0 = a->state_in; p->hT = a->state_out;
   p->done = a->done; p->done_n = a->done_stride_n; p->done_l = a->done_stride_l;
   p->ckpt = a->checkpoints;
@@ -1024,9 +1024,9 @@ extern "C" int srwm_b200_scan_backward(const srwm_b200_scan_args* a, const srwm_
   const int64_t need = 4 * srwm::scan_bwd_scratch(p, nullptr);
   if (!a->scratch || a->scratch_bytes < need) return SRWM_B200_ERR_NULL;
   srwm::scan_bwd_scratch(p, (float*)a->scratch);
-  p.dy = scan_rows(g->dy, Dg, es); p.du = scan_rows(g->du, Dg, es);
-  p.ddelta = scan_rows(g->ddelta, Dg, es); p.dz = scan_rows(g->dz, Dg, es);
-  p.dB = scan_rows(g->dB, a->S, es); p.dC = scan_rows(g->dC, a->S, es);
+  p.dy = scan_rows(g->dy, Dg, es, &p.vec); p.du = scan_rows(g->du, Dg, es, &p.vec);
+  p.ddelta = scan_rows(g->ddelta, Dg, es, &p.vec); p.dz = scan_rows(g->dz, Dg, es, &p.vec);
+  p.dB = scan_rows(g->dB, a->S, es, &p.vec); p.dC = scan_rows(g->dC, a->S, es, &p.vec);
   p.dhT = g->dstate_out; p.dh0 = g->dstate_in; p.dA = g->dA; p.dskip = g->dskip; p.dbias = g->ddelta_bias;
   return cuda_result(srwm::scan_backward(p, (cudaStream_t)stream));
 }
@@ -1048,8 +1048,9 @@ static int conv_params(const srwm_b200_conv_args* a, srwm::ConvParams* p) {
     if (off(d, 4)) return SRWM_B200_ERR_ALIGN;
   p->bf16 = a->io_dtype == SRWM_B200_BF16;
   p->silu = a->silu != 0;
-  p->x = scan_rows(a->x, a->D, es); p->y = scan_rows(a->y, a->D, es);
-  p->s0 = scan_rows(a->state_in, a->D, es); p->sT = scan_rows(a->state_out, a->D, es);
+  p->vec = 1;
+  p->x = scan_rows(a->x, a->D, es, &p->vec); p->y = scan_rows(a->y, a->D, es, &p->vec);
+  p->s0 = scan_rows(a->state_in, a->D, es, &p->vec); p->sT = scan_rows(a->state_out, a->D, es, &p->vec);
   p->w = a->w; p->bias = a->bias;
   p->done = a->done; p->done_n = a->done_stride_n; p->done_l = a->done_stride_l;
   return 0;
@@ -1082,8 +1083,8 @@ extern "C" int srwm_b200_conv_backward(const srwm_b200_conv_args* a, const srwm_
     if (off(d, es)) return SRWM_B200_ERR_ALIGN;
   for (const void* d : {(const void*)g->dw, (const void*)g->dbias, (const void*)g->scratch})
     if (off(d, 4)) return SRWM_B200_ERR_ALIGN;
-  p.dy = scan_rows(g->dy, a->D, es); p.dx = scan_rows(g->dx, a->D, es);
-  p.dsT = scan_rows(g->dstate_out, a->D, es); p.ds0 = scan_rows(g->dstate_in, a->D, es);
+  p.dy = scan_rows(g->dy, a->D, es, &p.vec); p.dx = scan_rows(g->dx, a->D, es, &p.vec);
+  p.dsT = scan_rows(g->dstate_out, a->D, es, &p.vec); p.ds0 = scan_rows(g->dstate_in, a->D, es, &p.vec);
   p.dw = g->dw; p.dbias = g->dbias; p.part = (float*)g->scratch;
   return cuda_result(srwm::conv_backward(p, (cudaStream_t)stream));
 }

@@ -3,7 +3,7 @@
 // with the K - 1 inputs before the call carried as a state, and none read across an episode's start.
 //
 // Bound by HBM: one read and one write of [N, L, D].  A thread takes four channels and up to 16 steps in time order, its window in
-// registers, loads four steps ahead; the K - 1 steps in front of its own come from L2.
+// registers; the K - 1 steps in front of its own come from L2.
 #include <type_traits>
 
 #include "chain.h"
@@ -36,18 +36,18 @@ __device__ __forceinline__ bool starts(const ConvParams& p, int n, int t) {
   return p.done && p.done[n * p.done_n + (long long)t * p.done_l] != 0;
 }
 // x_t of the call, or of the state in front of it
-template <typename T, int K>
-__device__ __forceinline__ Chan4 input(const ConvParams& p, int n, int t, int d, int valid) {
-  const ScanRows& r = t >= 0 ? p.x : p.s0;
-  if (r.p == nullptr) return Chan4();
-  const T* ptr = reinterpret_cast<const T*>(r.p) + n * r.sn + (long long)(t >= 0 ? t : t + K - 1) * r.sl + d;
-  Quad<T> qd;
-  qd.fetch(ptr, r.vec, valid);
-  return Chan4(qd.get(ptr, r.vec, valid));
+template <typename T, int K, bool VEC>
+__device__ __forceinline__ Quad<T, VEC> input(const ConvParams& p, int n, int t, int d, int valid) {
+  const bool before = t < 0;
+  const char* base = before ? p.s0.p : p.x.p;
+  const long long at = before ? n * p.s0.sn + (t + K - 1) * p.s0.sl : n * p.x.sn + t * p.x.sl;
+  Quad<T, VEC> q;
+  q.fetch(reinterpret_cast<const T*>(base) + at + d, base ? valid : 0);
+  return q;
 }
 
-// TS: steps of a thread
-template <typename T, int K, int TS>
+// TS: steps of a thread, whose loads are all on their way before the first is used
+template <typename T, bool VEC, int K, int TS, bool DONE>
 __global__ void __launch_bounds__(128) conv_fwd_kernel(const ConvParams p) {
   chained();
   const int quads = (p.D + 3) / 4, chunks = p.L == 0 ? 1 : (p.L + TS - 1) / TS;
@@ -56,73 +56,58 @@ __global__ void __launch_bounds__(128) conv_fwd_kernel(const ConvParams p) {
   const long long n_ = id / quads / chunks;
   if (n_ >= p.N) return;
   const int n = (int)n_, t0 = chunk * TS, t_end = min(p.L, t0 + TS);
+  const T* px = reinterpret_cast<const T*>(p.x.p) + n * p.x.sn + t0 * p.x.sl + d;
+  T* py = reinterpret_cast<T*>(p.y.p) + n * p.y.sn + t0 * p.y.sl + d;
+  Quad<T, VEC> row[TS], past[K];
+  bool cut[TS];
+#pragma unroll
+  for (int k = 0; k < TS; ++k) {
+    row[k].fetch(px + k * p.x.sl, t0 + k < t_end ? valid : 0);
+    if (DONE) cut[k] = t0 + k < t_end && starts(p, n, t0 + k);
+  }
+#pragma unroll
+  for (int j = 1; j < K; ++j) past[j] = input<T, K, VEC>(p, n, t0 - K + j, d, valid);
   float w[K][4], b[4];
   load_taps<K>(p, d, valid, w, b);
   Chan4 win[K];       // x_{t-K+1} .. x_t
 #pragma unroll
   for (int j = 1; j < K; ++j) {
     const int t = t0 - K + j;
-    win[j] = input<T, K>(p, n, t, d, valid);
-    if (t >= 0 && starts(p, n, t)) {
+    win[j] = Chan4(past[j].get());
+    if (DONE && t >= 0 && starts(p, n, t)) {
 #pragma unroll
       for (int k = 1; k < j; ++k) win[k] = Chan4();
     }
   }
-  constexpr int AH = TS < 4 ? TS : 4;       // steps loaded at a time
-  const T* px = reinterpret_cast<const T*>(p.x.p) + n * p.x.sn + d;
-  T* py = reinterpret_cast<T*>(p.y.p) + n * p.y.sn + d;
-  Quad<T> next[AH];
-  bool cut[AH];
 #pragma unroll
-  for (int k = 0; k < AH; ++k) {
-    const int t = t0 + k;
-    next[k].fetch(px + t * p.x.sl, p.x.vec, t < t_end ? valid : 0);
-    cut[k] = t < t_end && starts(p, n, t);
-  }
+  for (int k = 0; k < TS; ++k) {
+    if (t0 + k >= t_end) break;
 #pragma unroll
-  for (int g = 0; g < TS; g += AH) {
-    Quad<T> cur[AH];
-    bool fresh[AH];
+    for (int j = 0; j + 1 < K; ++j) win[j] = DONE && cut[k] ? Chan4() : win[j + 1];
+    win[K - 1] = Chan4(row[k].get());
+    Chan4 y;
 #pragma unroll
-    for (int k = 0; k < AH; ++k) {
-      cur[k] = next[k];
-      fresh[k] = cut[k];
-      const int t = t0 + g + AH + k;
-      if (g + AH < TS) {
-        next[k].fetch(px + t * p.x.sl, p.x.vec, t < t_end ? valid : 0);
-        cut[k] = t < t_end && starts(p, n, t);
-      }
+    for (int i = 0; i < 4; ++i) {
+      float a = b[i];
+#pragma unroll
+      for (int j = 0; j < K; ++j) a = fmaf(w[j][i], win[j].v[i], a);
+      y.v[i] = p.silu ? a * sigmoid(a) : a;
     }
-#pragma unroll
-    for (int k = 0; k < AH; ++k) {
-      const int t = t0 + g + k;
-      if (t >= t_end) break;
-#pragma unroll
-      for (int j = 0; j + 1 < K; ++j) win[j] = fresh[k] ? Chan4() : win[j + 1];
-      win[K - 1] = Chan4(cur[k].get(px + t * p.x.sl, p.x.vec, valid));
-      Chan4 y;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float a = b[i];
-#pragma unroll
-        for (int j = 0; j < K; ++j) a = fmaf(w[j][i], win[j].v[i], a);
-        y.v[i] = p.silu ? a * sigmoid(a) : a;
-      }
-      put4(py + t * p.y.sl, p.y.vec, valid, y.f4());
-    }
+    put4<VEC>(py + k * p.y.sl, valid, y.f4());
   }
   if (t_end == p.L && p.sT.p) {
     T* ps = reinterpret_cast<T*>(p.sT.p) + n * p.sT.sn + d;
 #pragma unroll
-    for (int j = 1; j < K; ++j) put4(ps + (j - 1) * p.sT.sl, p.sT.vec, valid, win[j].f4());
+    for (int j = 1; j < K; ++j) put4<VEC>(ps + (j - 1) * p.sT.sl, valid, win[j].f4());
   }
 }
 
 // A warp takes 32 quads of channels and a chunk of TS steps at a time, the block's four warps one chunk after another's; the sums of dw
 // and dbias stay with the threads.  What the outputs behind the chunk give to its inputs comes from TS + K - 1 steps of dy.
-template <typename T, int K, int TS>
+template <typename T, bool VEC, int K, int TS, bool DONE>
 __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
   __shared__ float4 red[4][32];
+  constexpr int ALL = TS + K - 1, AHEAD = 4;      // steps of a chunk, and how many of them are on their way
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int d = ((int)blockIdx.x * 32 + lane) * 4, valid = max(0, min(4, p.D - d));
   const int chunks = (p.L + TS - 1) / TS;
@@ -137,15 +122,31 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
   }
   for (long long u = (long long)blockIdx.y * 4 + warp; u < units; u += (long long)gridDim.y * 4) {
     if (valid == 0) break;
-    const int n = (int)(u / chunks), t0 = (int)(u % chunks) * TS, t_end = min(p.L, t0 + TS);
-    // from the chunk's first step (the state's first row in front of the first chunk) on: dx[s] is whole once the step K - 1 behind it is done
+    const int n = (int)(u / chunks), t0 = (int)(u % chunks) * TS;
+    const T* px = reinterpret_cast<const T*>(p.x.p) + n * p.x.sn + t0 * p.x.sl + d;
+    const T* py = reinterpret_cast<const T*>(p.dy.p) + n * p.dy.sn + t0 * p.dy.sl + d;
+    T* ox = reinterpret_cast<T*>(p.dx.p) + n * p.dx.sn + t0 * p.dx.sl + d;
+    Quad<T, VEC> rx[AHEAD], ry[AHEAD], past[K];
+#pragma unroll
+    for (int j = 1; j < K; ++j) past[j] = input<T, K, VEC>(p, n, t0 - K + j, d, valid);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int v = t0 + k < p.L ? valid : 0;
+      rx[k].fetch(px, v);
+      ry[k].fetch(py, v);
+      px += p.x.sl;
+      py += p.dy.sl;
+    }
+    // From the chunk's first step on, K - 1 steps beyond its last: dx[s] (of the state's rows too, in the first chunk) is whole
+    // once the step K - 1 behind it is done.  Steps beyond the call's end have no gradient.
+    const bool last = t0 + TS > p.L - (K - 1) && p.dsT.p != nullptr;      // some of the inputs are in the state behind the call
     Chan4 win[K], acc[K];       // acc[j]: of the input at t - K + 1 + j
     int age = K - 1;            // steps since the episode's start, as far as they matter
 #pragma unroll
     for (int j = 1; j < K; ++j) {
       const int t = t0 - K + j;
-      win[j] = input<T, K>(p, n, t, d, valid);
-      if (t >= 0) {
+      win[j] = Chan4(past[j].get());
+      if (DONE && t >= 0) {
         const bool cut = starts(p, n, t);
         if (cut) {
 #pragma unroll
@@ -154,80 +155,65 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
         age = cut ? 0 : min(K - 1, age + 1);
       }
     }
-    const T* px = reinterpret_cast<const T*>(p.x.p) + n * p.x.sn + d;
-    const T* py = reinterpret_cast<const T*>(p.dy.p) + n * p.dy.sn + d;
-    T* ox = reinterpret_cast<T*>(p.dx.p) + n * p.dx.sn + d;
-    constexpr int AH = 4;
-    Quad<T> nx[AH], ny[AH];
-    const int t_all = min(p.L, t_end + K - 1);     // steps whose outputs read the chunk's inputs
+    // what the state behind the call gives to the input at s
+    auto carried = [&](int s) {
+      Quad<T, VEC> q;
+      bool kept = last && s >= p.L - (K - 1) && s < p.L;
+      if (DONE && kept)
+        for (int r = max(s + 1, 0); r < p.L; ++r) kept = kept && !starts(p, n, r);
+      q.fetch(reinterpret_cast<const T*>(p.dsT.p) + n * p.dsT.sn + (long long)(s - (p.L - (K - 1))) * p.dsT.sl + d, kept ? valid : 0);
+      return Chan4(q.get());
+    };
+    if (last) {
 #pragma unroll
-    for (int k = 0; k < AH; ++k) {
-      const int t = t0 + k, v = t < t_all ? valid : 0;
-      nx[k].fetch(px + t * p.x.sl, p.x.vec, v);
-      ny[k].fetch(py + t * p.dy.sl, p.dy.vec, v);
+      for (int j = 1; j < K; ++j) acc[j] = carried(t0 - K + j);
     }
-    for (int g = t0; g < t_end + K - 1; g += AH) {
-      Quad<T> cx[AH], cy[AH];
 #pragma unroll
-      for (int k = 0; k < AH; ++k) {
-        cx[k] = nx[k];
-        cy[k] = ny[k];
-        const int t = g + AH + k, v = t < t_all ? valid : 0;
-        nx[k].fetch(px + t * p.x.sl, p.x.vec, v);
-        ny[k].fetch(py + t * p.dy.sl, p.dy.vec, v);
+    for (int k = 0; k < ALL; ++k) {
+      const int t = t0 + k;
+      if (t >= p.L + K - 1) break;
+#pragma unroll
+      for (int j = 0; j + 1 < K; ++j) acc[j] = acc[j + 1];
+      acc[K - 1] = last ? carried(t) : Chan4();
+      const bool fresh = DONE && t < p.L && starts(p, n, t);
+      if (DONE) age = fresh ? 0 : min(K - 1, age + 1);
+#pragma unroll
+      for (int j = 0; j + 1 < K; ++j) win[j] = DONE && fresh ? Chan4() : win[j + 1];
+      win[K - 1] = Chan4(rx[k % AHEAD].get());
+      const Chan4 go(ry[k % AHEAD].get());
+      if (k + AHEAD < ALL) {
+        const int v = t + AHEAD < p.L ? valid : 0;
+        rx[k % AHEAD].fetch(px, v);
+        ry[k % AHEAD].fetch(py, v);
+        px += p.x.sl;
+        py += p.dy.sl;
       }
 #pragma unroll
-      for (int k = 0; k < AH; ++k) {
-        const int t = g + k;
-        if (t >= t_end + K - 1) break;
+      for (int i = 0; i < 4; ++i) {
+        float gp = go.v[i];
+        if (p.silu) {
+          float a = b[i];
 #pragma unroll
-        for (int j = 0; j + 1 < K; ++j) acc[j] = acc[j + 1];
-        acc[K - 1] = Chan4();
-        if (t < p.L) {
-          const bool fresh = starts(p, n, t);
-          age = fresh ? 0 : min(K - 1, age + 1);
-#pragma unroll
-          for (int j = 0; j + 1 < K; ++j) win[j] = fresh ? Chan4() : win[j + 1];
-          win[K - 1] = Chan4(cx[k].get(px + t * p.x.sl, p.x.vec, valid));
-          const Chan4 go(cy[k].get(py + t * p.dy.sl, p.dy.vec, valid));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float a = b[i];
-#pragma unroll
-            for (int j = 0; j < K; ++j) a = fmaf(w[j][i], win[j].v[i], a);
-            float gp = go.v[i];
-            if (p.silu) {
-              const float sg = sigmoid(a);
-              gp *= sg * fmaf(a, 1.f - sg, 1.f);
-            }
-#pragma unroll
-            for (int j = 0; j < K; ++j)
-              if (K - 1 - j <= age) acc[j].v[i] = fmaf(w[j][i], gp, acc[j].v[i]);
-            if (t < t_end) {
-              db[i] += gp;
-#pragma unroll
-              for (int j = 0; j < K; ++j) dw[j][i] = fmaf(gp, win[j].v[i], dw[j][i]);
-            }
-          }
+          for (int j = 0; j < K; ++j) a = fmaf(w[j][i], win[j].v[i], a);
+          const float sg = sigmoid(a);
+          gp *= sg * fmaf(a, 1.f - sg, 1.f);
+          if (t >= p.L) gp = 0.f;      // (whatever the window holds)
         }
-        const int s = t - (K - 1);      // the input whose gradient is whole now
-        if (s >= t0 || t0 == 0) {
-          Chan4 o = acc[0];
-          if (s >= p.L - (K - 1) && p.dsT.p) {      // it is in the state behind the call, unless an episode began after it
-            bool kept = true;
-            for (int r = max(s + 1, 0); r < p.L; ++r) kept = kept && !starts(p, n, r);
-            if (kept) {
-              const T* pg = reinterpret_cast<const T*>(p.dsT.p) + n * p.dsT.sn + (long long)(s - (p.L - (K - 1))) * p.dsT.sl + d;
-              Quad<T> qd;
-              qd.fetch(pg, p.dsT.vec, valid);
-              const Chan4 gs(qd.get(pg, p.dsT.vec, valid));
 #pragma unroll
-              for (int i = 0; i < 4; ++i) o.v[i] += gs.v[i];
-            }
-          }
-          if (s >= t0) put4(ox + s * p.dx.sl, p.dx.vec, valid, o.f4());
-          else if (p.ds0.p) put4(reinterpret_cast<T*>(p.ds0.p) + n * p.ds0.sn + (long long)(s + K - 1) * p.ds0.sl + d, p.ds0.vec, valid, o.f4());
+        for (int j = 0; j < K; ++j)
+          if (!DONE || K - 1 - j <= age) acc[j].v[i] = fmaf(w[j][i], gp, acc[j].v[i]);
+        if (k < TS) {
+          db[i] += gp;
+#pragma unroll
+          for (int j = 0; j < K; ++j)
+            if (!DONE || K - 1 - j <= age) dw[j][i] = fmaf(gp, win[j].v[i], dw[j][i]);
         }
+      }
+      if (k >= K - 1) {
+        put4<VEC>(ox, t - (K - 1) < p.L ? valid : 0, acc[0].f4());
+        ox += p.dx.sl;
+      } else if (t0 == 0 && p.ds0.p) {
+        put4<VEC>(reinterpret_cast<T*>(p.ds0.p) + n * p.ds0.sn + k * p.ds0.sl + d, valid, acc[0].f4());
       }
     }
   }
@@ -253,54 +239,65 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
   }
 }
 
-// [parts][D][K + 1] -> dw [D][K], dbias [D]: 32 values a block, eight slices of the parts
-__global__ void __launch_bounds__(256) conv_sums_kernel(const float* part, int parts, int D, int K, float* dw, float* dbias) {
-  __shared__ float s[8][33];
-  const int c = threadIdx.x % 32, slice = threadIdx.x / 32, total = D * (K + 1), i = blockIdx.x * 32 + c;
+struct ConvSums {
+  const float* part;
+  float *dw, *dbias;
+  int parts, D, K;
+};
+// [parts][D][K + 1] -> dw [D][K], dbias [D]: 32 values a block, 32 slices of the parts
+__global__ void __launch_bounds__(1024) conv_sums_kernel(const ConvSums a) {
+  chained();
+  __shared__ float s[32][33];
+  const int c = threadIdx.x % 32, slice = threadIdx.x / 32, total = a.D * (a.K + 1);
+  int i = blockIdx.x * 32 + c;
   float t = 0.f;
   if (i < total) {
-#pragma unroll 4
-    for (int b = slice; b < parts; b += 8) t += part[(long long)b * total + i];
+#pragma unroll 8
+    for (int b = slice; b < a.parts; b += 32) t += a.part[(long long)b * total + i];
   }
   s[slice][c] = t;
   __syncthreads();
-  if (slice != 0 || i >= total) return;
-#pragma unroll
-  for (int k = 1; k < 8; ++k) t += s[k][c];
-  const int d = i / (K + 1), j = i % (K + 1);
-  if (j < K) dw[(long long)d * K + j] = t;
-  else if (dbias) dbias[d] = t;
+  t = allreduce_warp(s[c][slice]);
+  i = blockIdx.x * 32 + slice;
+  if (c != 0 || i >= total) return;
+  const int d = i / (a.K + 1), j = i % (a.K + 1);
+  if (j < a.K) a.dw[(long long)d * a.K + j] = t;
+  else if (a.dbias) a.dbias[d] = t;
 }
 
-template <typename T, int K>
+template <typename T, bool VEC, int K>
 cudaError_t fwd(const ConvParams& p, cudaStream_t s) {
   const long long quads = (p.D + 3) / 4;
   auto run = [&](auto ts) {
     constexpr int TS = decltype(ts)::value;
     const long long chunks = p.L == 0 ? 1 : (p.L + TS - 1) / TS, blocks = (quads * chunks * p.N + 127) / 128;
-    return launch_behind(conv_fwd_kernel<T, K, TS>, p, dim3((unsigned)blocks), 128, 0, s);
+    return p.done ? launch_behind(conv_fwd_kernel<T, VEC, K, TS, true>, p, dim3((unsigned)blocks), 128, 0, s)
+                  : launch_behind(conv_fwd_kernel<T, VEC, K, TS, false>, p, dim3((unsigned)blocks), 128, 0, s);
   };
   if (p.L <= 1) return run(std::integral_constant<int, 1>());
   return run(std::integral_constant<int, CONV_CHUNK>());
 }
-template <typename T, int K>
+template <typename T, bool VEC, int K>
 cudaError_t bwd(const ConvParams& p, cudaStream_t s) {
   const int parts = conv_parts(p);
-  conv_bwd_kernel<T, K, CONV_CHUNK><<<dim3((unsigned)((p.D + 127) / 128), (unsigned)parts), 128, 0, s>>>(p);
+  const dim3 grid((unsigned)((p.D + 127) / 128), (unsigned)parts);
+  if (p.done) conv_bwd_kernel<T, VEC, K, CONV_CHUNK, true><<<grid, 128, 0, s>>>(p);
+  else conv_bwd_kernel<T, VEC, K, CONV_CHUNK, false><<<grid, 128, 0, s>>>(p);
   if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-  conv_sums_kernel<<<(unsigned)((p.D * (K + 1) + 31) / 32), 256, 0, s>>>(p.part, parts, p.D, K, p.dw, p.dbias);
-  return cudaGetLastError();
+  return launch_behind(conv_sums_kernel, ConvSums{p.part, p.dw, p.dbias, parts, p.D, K}, dim3((unsigned)((p.D * (K + 1) + 31) / 32)), 1024, 0, s);
 }
+// f(element, VEC, K)
 template <typename F>
 cudaError_t by_type(const ConvParams& p, F f) {
-  auto taps = [&](auto t) {
+  auto taps = [&](auto t, auto vec) {
     switch (p.K) {
-      case 2: return f(t, std::integral_constant<int, 2>());
-      case 3: return f(t, std::integral_constant<int, 3>());
-      default: return f(t, std::integral_constant<int, 4>());
+      case 2: return f(t, vec, std::integral_constant<int, 2>());
+      case 3: return f(t, vec, std::integral_constant<int, 3>());
+      default: return f(t, vec, std::integral_constant<int, 4>());
     }
   };
-  return p.bf16 ? taps(__nv_bfloat16()) : taps(float());
+  if (p.bf16) return p.vec ? taps(__nv_bfloat16(), std::true_type()) : taps(__nv_bfloat16(), std::false_type());
+  return p.vec ? taps(float(), std::true_type()) : taps(float(), std::false_type());
 }
 
 }  // namespace
@@ -313,10 +310,10 @@ int conv_parts(const ConvParams& p) {
   return n < 1 ? 1 : (int)n;
 }
 cudaError_t conv_forward(const ConvParams& p, cudaStream_t s) {
-  return by_type(p, [&](auto t, auto k) { return fwd<decltype(t), decltype(k)::value>(p, s); });
+  return by_type(p, [&](auto t, auto v, auto k) { return fwd<decltype(t), decltype(v)::value, decltype(k)::value>(p, s); });
 }
 cudaError_t conv_backward(const ConvParams& p, cudaStream_t s) {
-  return by_type(p, [&](auto t, auto k) { return bwd<decltype(t), decltype(k)::value>(p, s); });
+  return by_type(p, [&](auto t, auto v, auto k) { return bwd<decltype(t), decltype(v)::value, decltype(k)::value>(p, s); });
 }
 
 }  // namespace srwm

@@ -11,7 +11,7 @@ constexpr int CONV_CHUNK = 16;     // steps of a thread at most
 
 struct ConvParams {
   int N, L, D, K;
-  int bf16, silu;
+  int bf16, silu, vec;             // vec: all rows' pieces of four channels are aligned to their size
   ScanRows x, y, s0, sT;           // [N, L, D]; the states [N, K-1, D], NULL: zeros / not wanted
   const float *w, *bias;           // [D, K], [D] or NULL
   const uint8_t* done;

@@ -282,18 +282,24 @@ PyObject* rms_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (list of tensors, max_norm or a negative number) -> norm; with a max_norm the tensors are scaled in place
+// (list of tensors, max_norm or a negative number, whether it is their .grad that is meant) -> norm; with a max_norm they are
+// scaled in place
 PyObject* grads_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arity(n, 2)) return nullptr;
+  if (!arity(n, 3)) return nullptr;
+  const bool of_params = PyObject_IsTrue(args[2]);
   const double max_norm = PyFloat_AsDouble(args[1]);
   if (max_norm == -1.0 && PyErr_Occurred()) return nullptr;
   if (!PyList_Check(args[0])) return declined();
-  std::vector<Tensor> ts((size_t)PyList_GET_SIZE(args[0]));
-  for (size_t i = 0; i < ts.size(); ++i) {
-    PyObject* o = PyList_GET_ITEM(args[0], (Py_ssize_t)i);
+  std::vector<Tensor> ts;
+  const Py_ssize_t count = PyList_GET_SIZE(args[0]);
+  ts.reserve((size_t)count);
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    PyObject* o = PyList_GET_ITEM(args[0], i);
     if (!plain(o)) return declined();
-    ts[i] = THPVariable_Unpack(o);
+    const Tensor& t = THPVariable_Unpack(o);
+    if (!of_params) ts.push_back(t);
+    else if (t.grad().defined()) ts.push_back(t.grad());
   }
   if (ts.empty() || !grads_ok(ts)) return declined();
   Tensor norm;

@@ -8,6 +8,8 @@
 // states of one channel in registers and walks the time axis; LN neighbouring lanes share a channel.  What belongs to a channel and
 // step (softplus, the gate) is formed once per tile of 16 steps x 32 channels, by the thread that loads it.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 #include "scan.h"
 
@@ -44,19 +46,35 @@ __device__ __forceinline__ float rcp(float x) {
 }
 constexpr float LOG2E = 1.4426950408889634f;
 
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-LOG2E * x)); }
-// max(x, 0) + log(1 + e), e = exp(-|x|) <= 1, as 2 atanh(e / (2 + e)): its series in s^2 <= 1/9 keeps the relative error of small
-// results (step sizes of 1e-3) near fp32's own, which a logarithm of 1 + e would not
+// max(x, 0) + log(1 + e), e = exp(-|x|): log(1 + e) / e as a polynomial (fitted for the least largest relative error on [0, 1]:
+// 3e-8), so that small results (step sizes of 1e-3) keep fp32's relative precision, and without a reciprocal: the special-function pipe has enough
+// to do.  Two at a time.
+__device__ __forceinline__ u64 softplus2(u64 x) {
+  float a, b;
+  unpack2(x, a, b);
+  const u64 e = pack2(ex2(-LOG2E * fabsf(a)), ex2(-LOG2E * fabsf(b)));
+  u64 p = dup2(0.0052326880395412445f);
+  p = fma2<true>(p, e, dup2(-0.029505213722586632f));
+  p = fma2<true>(p, e, dup2(0.07822591066360474f));
+  p = fma2<true>(p, e, dup2(-0.13663242757320404f));
+  p = fma2<true>(p, e, dup2(0.19106005132198334f));
+  p = fma2<true>(p, e, dup2(-0.2484298199415207f));
+  p = fma2<true>(p, e, dup2(0.3331909775733948f));
+  p = fma2<true>(p, e, dup2(-0.4999949336051941f));
+  p = fma2<true>(p, e, dup2(0.9999999403953552f));
+  // (fmaxf drops a NaN, which is in the other term)
+  return fma2<true>(p, e, pack2(fmaxf(a, 0.f), fmaxf(b, 0.f)));
+}
 __device__ __forceinline__ float softplus(float x) {
-  const float e = ex2(-LOG2E * fabsf(x)), s = e * rcp(2.f + e), q = s * s;
-  float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
-  p = fmaf(q, p, 1.f / 9.f);
-  p = fmaf(q, p, 1.f / 7.f);
-  p = fmaf(q, p, 1.f / 5.f);
-  p = fmaf(q, p, 1.f / 3.f);
-  p = fmaf(q, p, 1.f);
-  const float r = 2.f * s * p;
-  return x > 0.f ? x + r : (x == x ? r : x);
+  float r, other;
+  unpack2(softplus2(pack2(x, x)), r, other);
+  return r;
 }
 
 // Four neighbouring elements of a row, kept as they are loaded (a conversion would wait for the load)
@@ -78,40 +96,55 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162f
 __device__ __forceinline__ void narrow(float v, float* p) { *p = v; }
 __device__ __forceinline__ void narrow(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
 
-template <typename T>
+// VEC: every piece of four may be loaded and stored whole (otherwise by elements); a piece has four elements then, or none.
+// Loads are predicated, not behind branches, so that many are on their way at a time.
+template <typename T, bool VEC>
 struct Quad {
   typename Raw<T>::type raw;
-  // a row's piece ahead of time where it may be loaded whole; otherwise get() loads its elements
-  __device__ __forceinline__ void fetch(const T* p, int vec, int valid) {
-    if (vec && valid > 0) raw = *reinterpret_cast<const typename Raw<T>::type*>(p);
+  __device__ __forceinline__ void fetch(const T* p, int valid) {
+    raw = typename Raw<T>::type();
+    if (valid > 0) raw = *reinterpret_cast<const typename Raw<T>::type*>(p);
   }
-  __device__ __forceinline__ float4 get(const T* p, int vec, int valid) const {
-    if (valid <= 0) return make_float4(0.f, 0.f, 0.f, 0.f);
-    if (vec) return widen(raw);
-    float4 r = make_float4(to_float(p[0]), 0.f, 0.f, 0.f);
-    if (valid > 1) r.y = to_float(p[1]);
-    if (valid > 2) r.z = to_float(p[2]);
-    if (valid > 3) r.w = to_float(p[3]);
-    return r;
-  }
+  __device__ __forceinline__ float4 get() const { return widen(raw); }
 };
-__device__ __forceinline__ void put4(float* p, int vec, int valid, float4 v) {
-  if (vec) { *reinterpret_cast<float4*>(p) = v; return; }
-  p[0] = v.x;
-  if (valid > 1) p[1] = v.y;
-  if (valid > 2) p[2] = v.z;
-  if (valid > 3) p[3] = v.w;
-}
-__device__ __forceinline__ void put4(__nv_bfloat16* p, int vec, int valid, float4 v) {
-  if (vec) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(f32x2_to_bf16x2(v.x, v.y), f32x2_to_bf16x2(v.z, v.w));
-    return;
+template <typename T>
+struct Quad<T, false> {
+  T e[4];
+  __device__ __forceinline__ void fetch(const T* p, int valid) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      e[i] = T(0.f);
+      if (valid > i) e[i] = p[i];
+    }
   }
-  p[0] = __float2bfloat16_rn(v.x);
-  if (valid > 1) p[1] = __float2bfloat16_rn(v.y);
-  if (valid > 2) p[2] = __float2bfloat16_rn(v.z);
-  if (valid > 3) p[3] = __float2bfloat16_rn(v.w);
+  __device__ __forceinline__ float4 get() const { return make_float4(to_float(e[0]), to_float(e[1]), to_float(e[2]), to_float(e[3])); }
+};
+template <bool VEC>
+__device__ __forceinline__ void put4(float* p, int valid, float4 v) {
+  if constexpr (VEC) {
+    if (valid > 0) *reinterpret_cast<float4*>(p) = v;
+  } else {
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (valid > i) p[i] = e[i];
+  }
 }
+template <bool VEC>
+__device__ __forceinline__ void put4(__nv_bfloat16* p, int valid, float4 v) {
+  if constexpr (VEC) {
+    if (valid > 0) *reinterpret_cast<uint2*>(p) = make_uint2(f32x2_to_bf16x2(v.x, v.y), f32x2_to_bf16x2(v.z, v.w));
+  } else {
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (valid > i) p[i] = __float2bfloat16_rn(e[i]);
+  }
+}
+
+// Where a channel's value lies in a staged row of 16-byte pieces: a thread writes four neighbouring channels, a warp reads eight;
+// turned by one per eight channels both are free of conflicts
+__device__ __forceinline__ int swizzled(int ch) { return (ch & ~7) | ((ch + (ch >> 3)) & 7); }
 
 // Sums over a channel's LN lanes of LN steps' values: lane q gets step q's
 template <int LN>
@@ -181,10 +214,26 @@ __device__ __forceinline__ unsigned reset_bits(const ScanParams& p, int n, int t
   return __ballot_sync(0xffffffffu, r);
 }
 
-template <int S>
 inline int blocks_of(const ScanParams& p) {
   const int Dg = p.D / p.G;
   return (Dg + SCAN_CH - 1) / SCAN_CH * p.G;
+}
+
+// f(element, states, vec) as types
+template <typename T, bool VEC, typename F>
+inline cudaError_t by_states(const ScanParams& p, F& f) {
+  const std::bool_constant<VEC> vec;
+  switch (p.S) {
+    case 8: return f(T(), std::integral_constant<int, 8>(), vec);
+    case 16: return f(T(), std::integral_constant<int, 16>(), vec);
+    case 32: return f(T(), std::integral_constant<int, 32>(), vec);
+    default: return f(T(), std::integral_constant<int, 64>(), vec);
+  }
+}
+template <typename F>
+inline cudaError_t by_shape(const ScanParams& p, F f) {
+  if (p.bf16) return p.vec ? by_states<__nv_bfloat16, true>(p, f) : by_states<__nv_bfloat16, false>(p, f);
+  return p.vec ? by_states<float, true>(p, f) : by_states<float, false>(p, f);
 }
 
 }  // namespace scan

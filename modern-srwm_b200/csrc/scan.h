@@ -13,12 +13,12 @@ constexpr int SCAN_STEPS_DIRECT = 4;   // up to so many steps without gradients 
 struct ScanRows {               // [N, L, D] (or [N, L, G, S]), innermost dense; strides in elements
   char* p;
   long long sn, sl, sg;
-  int vec;                      // every row's pieces of four elements are aligned to their size
 };
 
 struct ScanParams {
   int N, L, D, G, S;
   int bf16, softplus;
+  int vec;                      // all rows' pieces of four elements are aligned to their size
   int nseg, seglen;             // pieces of the time axis (seglen a multiple of SCAN_TILE)
   ScanRows u, delta, z, y, B, C;
   const float *A, *skip, *bias, *h0;

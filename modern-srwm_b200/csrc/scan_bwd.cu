@@ -4,7 +4,8 @@
 //   dC_t = sum_d dy'_t h_t        dB_t = sum_d g_t Delta_t u_t        dA = sum_t Delta_t g_t a_t h_{t-1}
 //   du_t = D dy'_t + Delta_t (g_t . B_t)        dDelta_t = u_t (g_t . B_t) + sum_s A a_t h_{t-1} g_t
 // A CTA takes its 32 channels from the last step to the first.  The states in front of each eighth step are the forward's; within
-// eight steps they are formed again, a_t and a_t h_{t-1} staying in registers until the way back has used them.  Thirteen fp32
+// eight steps they are formed again, a_t and a_t h_{t-1} staying in registers until the way back has used them (four steps of them
+// where a thread has eight states: the first four are walked twice then).  Thirteen fp32
 // operations per state and step bind.  Sums over states go through a channel's lanes, sums over channels (dB, dC) through the
 // warp's other lanes and shared memory, and are added up over the CTAs by a second launch, in a fixed order.
 #include <type_traits>
@@ -15,12 +16,6 @@
 namespace srwm {
 namespace {
 using namespace scan;
-
-__device__ __forceinline__ u64 add2(u64 a, u64 b) {
-  u64 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 
 // Sums of eight values over a warp's LC channels: 8 / LC values stay with each lane, those from index `kept_of` on
 template <int LN, int LC>
@@ -48,24 +43,32 @@ struct BwdSmem {
   float2 gy[TT][CH];           // dy' twice
   float bc[2][TT][S];
   float gb[TT][PAD], sa[TT][PAD], yp[TT][PAD];
-  float part[WARPS][SCAN_CKPT][2][S];
+  float part[WARPS][TT][2][S];
 };
 
-template <typename T, int S>
-__global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_kernel(const ScanParams p) {
+// Steps whose a and a h stay in registers, and CTAs that a multiprocessor is to hold (168 registers a thread, or 128)
+template <int S>
+struct BwdPlan {
+  static constexpr int SUB = Shape<S>::ST == 8 ? 4 : 8, CTAS = S == 8 ? 4 : S == 64 ? 1 : 2;
+};
+
+template <typename T, int S, bool VEC>
+__global__ void __launch_bounds__(Shape<S>::NT, BwdPlan<S>::CTAS) scan_bwd_kernel(const ScanParams p) {
   using Sh = Shape<S>;
-  constexpr int TT = SCAN_TILE, CH = SCAN_CH, KT = SCAN_CKPT, NP = Sh::ST / 2, GS = 8 / Sh::ST, KEPT = 8 / Sh::LC;
+  constexpr int TT = SCAN_TILE, CH = SCAN_CH, KT = SCAN_CKPT, NP = Sh::ST / 2, GS = 8 / Sh::ST, KEPT = 8 / Sh::LC, SUB = BwdPlan<S>::SUB;
+  constexpr int WARPS = BwdSmem<S>::WARPS;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   BwdSmem<S>& sm = *reinterpret_cast<BwdSmem<S>*>(raw_smem);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, q = lane % Sh::LN, chl = warp * Sh::LC + lane / Sh::LN;
   const Place at(p, blockIdx.x);
   const int seg = blockIdx.y, t_first = seg * p.seglen, t_end = min(p.L, t_first + p.seglen);
+  const int t_last = t_first + (t_end - t_first - 1) / TT * TT;
   const bool mine = chl < at.left;
-  const int d = at.ch0 + chl;
+  const int d = at.ch0 + chl, here = swizzled(chl);
 
   const bool loader = tid < TT * CH / 4;
-  const int row = tid / (CH / 4), col = tid % (CH / 4) * 4, valid = loader ? min(4, at.left - col) : 0;
-  auto rows = [&](const ScanRows& w) { return reinterpret_cast<T*>(w.p) + at.n * w.sn + at.ch0 + col; };
+  const int row = tid / (CH / 4), col = tid % (CH / 4) * 4, valid = loader ? max(0, min(4, at.left - col)) : 0;
+  auto rows = [&](const ScanRows& w) { return reinterpret_cast<T*>(w.p) + at.n * w.sn + (t_last + row) * w.sl + at.ch0 + col; };
   const T *pu = rows(p.u), *pd = rows(p.delta), *pz = rows(p.z), *py = rows(p.dy);
   T *ou = rows(p.du), *od = rows(p.ddelta), *oz = rows(p.dz);
   const bool gate = p.z.p != nullptr;
@@ -76,36 +79,37 @@ __global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_kernel(const ScanParams
     skip[i] = i < valid && p.skip ? p.skip[at.ch0 + col + i] : 0.f;
     sum_skip[i] = sum_bias[i] = 0.f;
   }
-  Quad<T> ru, rd, rz, ry, rbc[Sh::NQ];
   const T* pbc[Sh::NQ];
   long long lbc[Sh::NQ];
-  int rbc_row[Sh::NQ], vbc[Sh::NQ];
-  float* sbc[Sh::NQ];
+  int rbc[Sh::NQ];
 #pragma unroll
   for (int i = 0; i < Sh::NQ; ++i) {
     const int id = tid + i * Sh::NT, c = id % (S / 4) * 4, r = id / (S / 4) % TT;
     const bool second = id >= TT * S / 4;
-    pbc[i] = second ? reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + c
-                    : reinterpret_cast<const T*>(p.B.p) + at.n * p.B.sn + at.g * p.B.sg + c;
-    lbc[i] = second ? p.C.sl : p.B.sl;
-    vbc[i] = second ? p.C.vec : p.B.vec;
-    rbc_row[i] = id < Sh::QUADS ? r : p.L;
-    sbc[i] = &sm.bc[second][r][c];
+    lbc[i] = (second ? p.C.sl : p.B.sl) * TT;
+    pbc[i] = second ? reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + (t_last + r) * p.C.sl + c
+                    : reinterpret_cast<const T*>(p.B.p) + at.n * p.B.sn + at.g * p.B.sg + (t_last + r) * p.B.sl + c;
+    rbc[i] = id < Sh::QUADS ? r : p.L;
   }
-  auto fetch = [&](int t0) {
-    const int t = t0 + row, v = t < t_end ? valid : 0;
-    ru.fetch(pu + t * p.u.sl, p.u.vec, v);
-    rd.fetch(pd + t * p.delta.sl, p.delta.vec, v);
-    ry.fetch(py + t * p.dy.sl, p.dy.vec, v);
-    if (gate) rz.fetch(pz + t * p.z.sl, p.z.vec, v);
+  Quad<T, VEC> fu, fd, fz, fy, fbc[Sh::NQ];
+  auto fetch = [&](int t0) {      // tiles are asked for in order, the last first
+    const int v = t0 + row < t_end ? valid : 0;
+    fu.fetch(pu, v);
+    fd.fetch(pd, v);
+    fy.fetch(py, v);
+    if (gate) fz.fetch(pz, v);
+    pu -= TT * p.u.sl; pd -= TT * p.delta.sl; py -= TT * p.dy.sl; pz -= TT * p.z.sl;
 #pragma unroll
-    for (int i = 0; i < Sh::NQ; ++i)
-      if (t0 + rbc_row[i] < t_end) rbc[i].fetch(pbc[i] + (t0 + rbc_row[i]) * lbc[i], vbc[i], 4);
+    for (int i = 0; i < Sh::NQ; ++i) {
+      fbc[i].fetch(pbc[i], t0 + rbc[i] < t_end ? 4 : 0);
+      pbc[i] -= lbc[i];
+    }
   };
 
   u64 A2[NP], gc[NP], dA[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) A2[i] = gc[i] = dA[i] = 0ull;
+  if (t_first < t_end) fetch(t_last);
   const long long states = (long long)p.N * p.D * S, own = ((long long)at.n * p.D + d) * S;
   const int nck = (p.L + KT - 1) / KT;
   if (mine) {
@@ -114,6 +118,7 @@ __global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_kernel(const ScanParams
 #pragma unroll
     for (int i = 0; i < NP; ++i) A2[i] = mul2(A2[i], l2);
     if (p.dhT) load_states<Sh>(p.dhT + own, q, gc);
+#pragma unroll 4
     for (int i = p.nseg - 1; i > seg; --i) {      // the pieces behind, the last first
       u64 decay[NP], end[NP];
       load_states<Sh>(p.carry + (2 * i - 2) * states + own, q, end);
@@ -124,57 +129,68 @@ __global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_kernel(const ScanParams
   }
   const int kept = kept_of<Sh::LN, Sh::LC>(lane), kept_step = kept / Sh::ST, kept_j = kept % Sh::ST;
   const int kept_state = Sh::first(q, kept_j / 4) + (Sh::ST >= 4 ? kept_j % 4 : kept_j);
+  float* part_mine = &sm.part[warp][kept_step][0][kept_state];
 
-  const int t_last = t_first + (t_end - t_first - 1) / TT * TT;
-  if (t_first < t_end) fetch(t_last);
   for (int t0 = t_last; t0 >= t_first; t0 -= TT) {
     const int steps = min(TT, t_end - t0);
-    float4 u4, z4, r4, y4;
+    // the states in front of the tile's two halves
+    u64 ck[2][NP];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) ck[k][i] = 0ull;
+      if (mine && k * KT < steps) load_states<Sh>(p.ckpt + (((long long)at.n * nck + t0 / KT + k) * p.D + d) * S, q, ck[k]);
+    }
+    const Quad<T, VEC> qu = fu, qd = fd, qz = fz, qy = fy;
+    u64 dl2[2], g2v[2];      // Delta and dy' of this thread's piece
+    dl2[0] = dl2[1] = g2v[0] = g2v[1] = 0ull;
     if (loader) {
-      const int t = t0 + row, v = t < t_end ? valid : 0;
-      u4 = ru.get(pu + t * p.u.sl, p.u.vec, v);
-      r4 = rd.get(pd + t * p.delta.sl, p.delta.vec, v);
-      y4 = ry.get(py + t * p.dy.sl, p.dy.vec, v);
-      z4 = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (gate) z4 = rz.get(pz + t * p.z.sl, p.z.vec, v);
-      const float us[4] = {u4.x, u4.y, u4.z, u4.w}, zs[4] = {z4.x, z4.y, z4.z, z4.w};
-      float rs[4] = {r4.x, r4.y, r4.z, r4.w}, gs[4] = {y4.x, y4.y, y4.z, y4.w};
+      const float4 u4 = qu.get(), r4 = qd.get(), y4 = qy.get();
+      dl2[0] = add2(pack2(r4.x, r4.y), pack2(bias[0], bias[1]));
+      dl2[1] = add2(pack2(r4.z, r4.w), pack2(bias[2], bias[3]));
+      if (p.softplus) {
+        dl2[0] = softplus2(dl2[0]);
+        dl2[1] = softplus2(dl2[1]);
+      }
+      const u64 xlo = mul2(dl2[0], pack2(u4.x, u4.y)), xhi = mul2(dl2[1], pack2(u4.z, u4.w));
+      float dl[4], du[4], g[4] = {y4.x, y4.y, y4.z, y4.w};
+      unpack2(dl2[0], dl[0], dl[1]); unpack2(dl2[1], dl[2], dl[3]);
+      unpack2(xlo, du[0], du[1]); unpack2(xhi, du[2], du[3]);
+      if (gate) {
+        const float4 z4 = qz.get();
+        g[0] *= z4.x * sigmoid(z4.x); g[1] *= z4.y * sigmoid(z4.y); g[2] *= z4.z * sigmoid(z4.z); g[3] *= z4.w * sigmoid(z4.w);
+      }
+      g2v[0] = pack2(g[0], g[1]); g2v[1] = pack2(g[2], g[3]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        rs[i] += bias[i];
-        float dl = p.softplus ? softplus(rs[i]) : rs[i];
-        dl = i < v ? dl : 0.f;
-        const float du = dl * us[i], g = gate ? gs[i] * zs[i] * sigmoid(zs[i]) : gs[i];
-        sm.dd[row][col + i] = make_float4(dl, dl, du, du);
-        sm.gy[row][col + i] = make_float2(g, g);
+        sm.dd[row][swizzled(col + i)] = make_float4(dl[i], dl[i], du[i], du[i]);
+        sm.gy[row][swizzled(col + i)] = make_float2(g[i], g[i]);
       }
-      r4 = make_float4(rs[0], rs[1], rs[2], rs[3]);
     }
 #pragma unroll
-    for (int i = 0; i < Sh::NQ; ++i)
-      if (t0 + rbc_row[i] < t_end)
-        *reinterpret_cast<float4*>(sbc[i]) = rbc[i].get(pbc[i] + (t0 + rbc_row[i]) * lbc[i], vbc[i], 4);
+    for (int i = 0; i < Sh::NQ; ++i) {
+      const int id = tid + i * Sh::NT;
+      if (id < Sh::QUADS) *reinterpret_cast<float4*>(&sm.bc[0][0][0] + id * 4) = fbc[i].get();
+    }
     const unsigned resets = reset_bits(p, at.n, t0, steps);
     __syncthreads();
     if (t0 - TT >= t_first) fetch(t0 - TT);
 
-    auto half = [&](auto whole, int s0) {       // eight steps from s0 of the tile
+    // SUB steps from s0 of the tile, h the state in front of them
+    auto steps_of = [&](auto whole, int s0, u64* h) __attribute__((always_inline)) {
       constexpr bool WHOLE = decltype(whole)::value;
-      u64 a[KT][NP], ah[KT][NP], h[NP];
-#pragma unroll
-      for (int i = 0; i < NP; ++i) h[i] = 0ull;
-      if (mine) load_states<Sh>(p.ckpt + (((long long)at.n * nck + (t0 + s0) / KT) * p.D + d) * S, q, h);
+      u64 a[SUB][NP], ah[SUB][NP];
       float yv[Sh::LN], dc[8];
 #pragma unroll
-      for (int k = 0; k < KT; ++k) {
+      for (int k = 0; k < SUB; ++k) {
         const int t = s0 + k;
         float* dck = dc + k % GS * Sh::ST;
         yv[k % Sh::LN] = 0.f;
 #pragma unroll
         for (int i = 0; i < Sh::ST; ++i) dck[i] = 0.f;
         if (WHOLE || t < steps) {
-          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sm.dd[t][chl]);
-          const u64 g2 = *reinterpret_cast<const u64*>(&sm.gy[t][chl]);
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sm.dd[t][here]);
+          const u64 g2 = *reinterpret_cast<const u64*>(&sm.gy[t][here]);
           const bool fresh = !WHOLE && (resets >> t & 1u);
           u64 b2[NP], c2[NP], acc = 0ull;
           load_states<Sh>(&sm.bc[0][t][0], q, b2);
@@ -192,25 +208,29 @@ __global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_kernel(const ScanParams
         }
         if (k % GS == GS - 1) {
           channels_to_lanes<Sh::LN, Sh::LC>(dc, lane);
+          float* o = part_mine + (s0 + k - (GS - 1)) * 2 * S + S;
 #pragma unroll
-          for (int i = 0; i < KEPT; ++i) sm.part[warp][k - (GS - 1) + kept_step][1][kept_state + i] = dc[i];
+          for (int i = 0; i < KEPT; ++i) o[i] = dc[i];
         }
-        if (gate && k % Sh::LN == Sh::LN - 1) {
+        // (a piece's last steps may be fewer than the lanes: the values are zero then, and the row is not read)
+        if (gate && (k % Sh::LN == Sh::LN - 1 || k == SUB - 1)) {
+#pragma unroll
+          for (int i = SUB; i < Sh::LN; ++i) yv[i] = 0.f;
           const float y = steps_to_lanes<Sh::LN>(yv, q);
-          sm.yp[s0 + k - (Sh::LN - 1) + q][chl] = y;
+          if (SUB >= Sh::LN || q < SUB) sm.yp[s0 + k - (SUB < Sh::LN ? SUB : Sh::LN) + 1 + q][chl] = y;
         }
       }
       float gbv[Sh::LN], sav[Sh::LN], db[8];
 #pragma unroll
-      for (int k = KT - 1; k >= 0; --k) {
+      for (int k = SUB - 1; k >= 0; --k) {
         const int t = s0 + k;
         float* dbk = db + k % GS * Sh::ST;
         gbv[k % Sh::LN] = sav[k % Sh::LN] = 0.f;
 #pragma unroll
         for (int i = 0; i < Sh::ST; ++i) dbk[i] = 0.f;
         if (WHOLE || t < steps) {
-          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sm.dd[t][chl]);
-          const u64 g2 = *reinterpret_cast<const u64*>(&sm.gy[t][chl]);
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sm.dd[t][here]);
+          const u64 g2 = *reinterpret_cast<const u64*>(&sm.gy[t][here]);
           u64 b2[NP], c2[NP], gb = 0ull, sa = 0ull;
           load_states<Sh>(&sm.bc[0][t][0], q, b2);
           load_states<Sh>(&sm.bc[1][t][0], q, c2);
@@ -229,60 +249,100 @@ __global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_kernel(const ScanParams
         }
         if (k % GS == 0) {
           channels_to_lanes<Sh::LN, Sh::LC>(db, lane);
+          float* o = part_mine + (s0 + k) * 2 * S;
 #pragma unroll
-          for (int i = 0; i < KEPT; ++i) sm.part[warp][k + kept_step][0][kept_state + i] = db[i];
+          for (int i = 0; i < KEPT; ++i) o[i] = db[i];
         }
         if (k % Sh::LN == 0) {
+#pragma unroll
+          for (int i = SUB; i < Sh::LN; ++i) gbv[i] = sav[i] = 0.f;
           const float g = steps_to_lanes<Sh::LN>(gbv, q), s = steps_to_lanes<Sh::LN>(sav, q);
-          sm.gb[s0 + k + q][chl] = g;
-          sm.sa[s0 + k + q][chl] = s * 0.6931471805599453f;      // (A2 has log2(e) in it)
+          if (SUB >= Sh::LN || q < SUB) {
+            sm.gb[s0 + k + q][chl] = g;
+            sm.sa[s0 + k + q][chl] = s * 0.6931471805599453f;      // (A2 has log2(e) in it)
+          }
         }
       }
     };
-    for (int s0 = TT - KT; s0 >= 0; s0 -= KT) {
-      if (s0 >= steps) continue;
-      if (steps == TT && resets == 0u) half(std::true_type(), s0);
-      else half(std::false_type(), s0);
-      __syncthreads();
-      // this CTA's share of dB and dC of the eight steps
-      for (int e = tid; e < KT * 2 * S; e += Sh::NT) {
-        const int s = e % S, arr = e / S % 2, k = e / (2 * S), t = t0 + s0 + k;
-        float v = sm.part[0][k][arr][s];
+    // eight steps at a time, the last first; where four stay in registers, the first four are walked on the way to the others
+    auto halves = [&](auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+#pragma unroll 1
+      for (int s0 = TT - SUB; s0 >= 0; s0 -= SUB) {
+        if (!WHOLE && s0 >= steps) continue;
+        u64 h[NP];
 #pragma unroll
-        for (int w = 1; w < BwdSmem<S>::WARPS; ++w) v += sm.part[w][k][arr][s];
-        const int per = ((p.D / p.G) + CH - 1) / CH, blk = (int)(blockIdx.x % (unsigned)per);
-        if (t < t_end) p.part_bc[((((long long)blk * 2 + arr) * p.N + at.n) * p.L + t) * p.G * S + at.g * S + s] = v;
+        for (int i = 0; i < NP; ++i) h[i] = s0 >= KT ? ck[1][i] : ck[0][i];
+        if (SUB < KT && s0 % KT != 0) {
+#pragma unroll
+          for (int k = 0; k < SUB; ++k) {
+            const int t = s0 - SUB + k;
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sm.dd[t][here]);
+            u64 b2[NP];
+            load_states<Sh>(&sm.bc[0][t][0], q, b2);
+            const bool fresh = !WHOLE && (resets >> t & 1u);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+              u64 a = exp2_pair(mul2(x.x, A2[i]));
+              if (fresh) a = h[i] = 0ull;
+              h[i] = add2(mul2(a, h[i]), mul2(x.y, b2[i]));
+            }
+          }
+        }
+        steps_of(whole, s0, h);
       }
-      __syncthreads();
+    };
+    if (steps == TT && resets == 0u) halves(std::true_type());
+    else halves(std::false_type());
+    __syncthreads();
+    {   // this CTA's share of dB and dC
+      const int per = ((p.D / p.G) + CH - 1) / CH, blk = (int)(blockIdx.x % (unsigned)per);
+#pragma unroll
+      for (int e = tid; e < TT * 2 * S / 4; e += Sh::NT) {
+        const int s = e % (S / 4) * 4, arr = e / (S / 4) % 2, t = e / (S / 2);
+        float4 v = *reinterpret_cast<const float4*>(&sm.part[0][t][arr][s]);
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) {
+          const float4 o = *reinterpret_cast<const float4*>(&sm.part[w][t][arr][s]);
+          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        }
+        if (t < steps)
+          *reinterpret_cast<float4*>(p.part_bc + ((((long long)blk * 2 + arr) * p.N + at.n) * p.L + t0 + t) * p.G * S + at.g * S + s) = v;
+      }
     }
-    if (loader && t0 + row < t_end && valid > 0) {
-      const int t = t0 + row;
+    const int v = row < steps ? valid : 0;
+    if (v > 0) {
       const float4 gb4 = *reinterpret_cast<const float4*>(&sm.gb[row][col]), sa4 = *reinterpret_cast<const float4*>(&sm.sa[row][col]);
-      float4 yp4 = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (gate) yp4 = *reinterpret_cast<const float4*>(&sm.yp[row][col]);
-      const float us[4] = {u4.x, u4.y, u4.z, u4.w}, rs[4] = {r4.x, r4.y, r4.z, r4.w}, zs[4] = {z4.x, z4.y, z4.z, z4.w};
-      const float os[4] = {y4.x, y4.y, y4.z, y4.w}, gb[4] = {gb4.x, gb4.y, gb4.z, gb4.w}, sa[4] = {sa4.x, sa4.y, sa4.z, sa4.w};
-      const float yp[4] = {yp4.x, yp4.y, yp4.z, yp4.w};
-      float ru4[4], rd4[4], rz4[4];
+      const float4 u4 = qu.get(), r4 = qd.get();
+      const float us[4] = {u4.x, u4.y, u4.z, u4.w}, rs[4] = {r4.x, r4.y, r4.z, r4.w};
+      const float gb[4] = {gb4.x, gb4.y, gb4.z, gb4.w}, sa[4] = {sa4.x, sa4.y, sa4.z, sa4.w};
+      float dl[4], g[4], o1[4], o2[4];
+      unpack2(dl2[0], dl[0], dl[1]); unpack2(dl2[1], dl[2], dl[3]);
+      unpack2(g2v[0], g[0], g[1]); unpack2(g2v[1], g[2], g[3]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float g = sm.gy[row][col + i].x, dl = sm.dd[row][col + i].x;
-        ru4[i] = fmaf(g, skip[i], dl * gb[i]);
-        float dr = fmaf(us[i], gb[i], sa[i]);
-        if (p.softplus) dr *= sigmoid(rs[i]);
-        rd4[i] = dr;
-        const float sg = sigmoid(zs[i]);
-        rz4[i] = os[i] * fmaf(skip[i], us[i], yp[i]) * sg * fmaf(zs[i], 1.f - sg, 1.f);
-        if (i < valid) {
-          sum_skip[i] = fmaf(g, us[i], sum_skip[i]);
-          sum_bias[i] += dr;
+        o1[i] = fmaf(g[i], skip[i], dl[i] * gb[i]);
+        o2[i] = fmaf(us[i], gb[i], sa[i]);
+        if (p.softplus) o2[i] *= sigmoid(rs[i] + bias[i]);
+        if (i < v) {
+          sum_skip[i] = fmaf(g[i], us[i], sum_skip[i]);
+          sum_bias[i] += o2[i];
         }
       }
-      put4(ou + t * p.du.sl, p.du.vec, valid, make_float4(ru4[0], ru4[1], ru4[2], ru4[3]));
-      put4(od + t * p.ddelta.sl, p.ddelta.vec, valid, make_float4(rd4[0], rd4[1], rd4[2], rd4[3]));
-      if (gate) put4(oz + t * p.dz.sl, p.dz.vec, valid, make_float4(rz4[0], rz4[1], rz4[2], rz4[3]));
+      put4<VEC>(ou, v, make_float4(o1[0], o1[1], o1[2], o1[3]));
+      put4<VEC>(od, v, make_float4(o2[0], o2[1], o2[2], o2[3]));
+      if (gate) {
+        const float4 yp4 = *reinterpret_cast<const float4*>(&sm.yp[row][col]), z4 = qz.get(), y4 = qy.get();
+        const float yp[4] = {yp4.x, yp4.y, yp4.z, yp4.w}, zs[4] = {z4.x, z4.y, z4.z, z4.w}, os[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float sg = sigmoid(zs[i]);
+          o1[i] = os[i] * fmaf(skip[i], us[i], yp[i]) * sg * fmaf(zs[i], 1.f - sg, 1.f);
+        }
+        put4<VEC>(oz, v, make_float4(o1[0], o1[1], o1[2], o1[3]));
+      }
     }
-    __syncthreads();
+    ou -= TT * p.du.sl; od -= TT * p.ddelta.sl; oz -= TT * p.dz.sl;
   }
   const long long slot = (long long)at.n * p.nseg + seg;
   if (mine) {
@@ -301,6 +361,7 @@ __global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_kernel(const ScanParams
   if (tid < 2 * CH) {
     const int c = tid % CH, which = tid / CH;
     float v = 0.f;
+#pragma unroll
     for (int r = 0; r < TT; ++r) v += which ? sm.sa[r][c] : sm.gb[r][c];
     if (c < at.left) p.part_v[(slot * 2 + which) * p.D + at.ch0 + c] = v;
   }
@@ -308,41 +369,73 @@ __global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_kernel(const ScanParams
 
 // What a piece of the time axis adds to the gradient of the state in front of it (from zero behind it), and the product of its
 // decays, for pieces 1 .. nseg - 1.
-template <typename T, int S>
+template <typename T, int S, bool VEC>
 __global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_carry_kernel(const ScanParams p) {
   using Sh = Shape<S>;
   constexpr int TT = SCAN_TILE, CH = SCAN_CH, NP = Sh::ST / 2, NQ = (Sh::QUADS / 2 + Sh::NT - 1) / Sh::NT;
-  __shared__ __align__(16) float4 dg[TT][CH];        // Delta twice, dy' twice
-  __shared__ __align__(16) float cs[TT][S];
+  __shared__ __align__(16) float4 dg[2][TT][CH];        // Delta twice, dy' twice
+  __shared__ __align__(16) float cs[2][TT][S];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, q = lane % Sh::LN, chl = warp * Sh::LC + lane / Sh::LN;
   const Place at(p, blockIdx.x);
   const int seg = blockIdx.y + 1, t_first = seg * p.seglen, t_end = min(p.L, t_first + p.seglen);
+  const int t_last = t_first + (t_end - t_first - 1) / TT * TT;
   const bool mine = chl < at.left;
-  const int d = at.ch0 + chl;
+  const int d = at.ch0 + chl, here = swizzled(chl);
   const bool loader = tid < TT * CH / 4;
-  const int row = tid / (CH / 4), col = tid % (CH / 4) * 4, valid = loader ? min(4, at.left - col) : 0;
-  auto rows = [&](const ScanRows& w) { return reinterpret_cast<const T*>(w.p) + at.n * w.sn + at.ch0 + col; };
+  const int row = tid / (CH / 4), col = tid % (CH / 4) * 4, valid = loader ? max(0, min(4, at.left - col)) : 0;
+  auto rows = [&](const ScanRows& w) { return reinterpret_cast<const T*>(w.p) + at.n * w.sn + (t_last + row) * w.sl + at.ch0 + col; };
   const T *pd = rows(p.delta), *pz = rows(p.z), *py = rows(p.dy);
   const bool gate = p.z.p != nullptr;
   float bias[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) bias[i] = i < valid && p.bias ? p.bias[at.ch0 + col + i] : 0.f;
-  const T* pc = reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg;
-  Quad<T> rd, rz, ry, rc[NQ];
+  const T* pc[NQ];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    const int id = tid + i * Sh::NT;
+    pc[i] = reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + (t_last + id / (S / 4)) * p.C.sl + id % (S / 4) * 4;
+  }
+  Quad<T, VEC> fd, fz, fy, fc[NQ];
   auto fetch = [&](int t0) {
-    const int t = t0 + row, v = t < t_end ? valid : 0;
-    rd.fetch(pd + t * p.delta.sl, p.delta.vec, v);
-    ry.fetch(py + t * p.dy.sl, p.dy.vec, v);
-    if (gate) rz.fetch(pz + t * p.z.sl, p.z.vec, v);
+    const int v = t0 + row < t_end ? valid : 0;
+    fd.fetch(pd, v);
+    fy.fetch(py, v);
+    if (gate) fz.fetch(pz, v);
+    pd -= TT * p.delta.sl; py -= TT * p.dy.sl; pz -= TT * p.z.sl;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      const int id = tid + i * Sh::NT, r = id / (S / 4);
-      if (r < TT && t0 + r < t_end) rc[i].fetch(pc + (t0 + r) * p.C.sl + id % (S / 4) * 4, p.C.vec, 4);
+      const int r = (tid + i * Sh::NT) / (S / 4);
+      fc[i].fetch(pc[i], r < TT && t0 + r < t_end ? 4 : 0);
+      pc[i] -= TT * p.C.sl;
+    }
+  };
+  auto stage = [&](int buf) {
+    if (loader) {
+      const float4 r4 = fd.get(), y4 = fy.get();
+      u64 lo = add2(pack2(r4.x, r4.y), pack2(bias[0], bias[1])), hi = add2(pack2(r4.z, r4.w), pack2(bias[2], bias[3]));
+      if (p.softplus) {
+        lo = softplus2(lo);
+        hi = softplus2(hi);
+      }
+      float dl[4], g[4] = {y4.x, y4.y, y4.z, y4.w};
+      unpack2(lo, dl[0], dl[1]); unpack2(hi, dl[2], dl[3]);
+      if (gate) {
+        const float4 z4 = fz.get();
+        g[0] *= z4.x * sigmoid(z4.x); g[1] *= z4.y * sigmoid(z4.y); g[2] *= z4.z * sigmoid(z4.z); g[3] *= z4.w * sigmoid(z4.w);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dg[buf][row][swizzled(col + i)] = make_float4(dl[i], dl[i], g[i], g[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int id = tid + i * Sh::NT;
+      if (id < Sh::QUADS / 2) *reinterpret_cast<float4*>(&cs[buf][0][0] + id * 4) = fc[i].get();
     }
   };
   u64 A2[NP], gc[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) A2[i] = gc[i] = 0ull;
+  if (t_first < t_end) fetch(t_last);
   if (mine) {
     load_states<Sh>(p.A + (long long)d * S, q, A2);
 #pragma unroll
@@ -350,46 +443,41 @@ __global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_carry_kernel(const Scan
   }
   float sum_d = 0.f;
   bool cut = false;
-  const int t_last = t_first + (t_end - t_first - 1) / TT * TT;
-  if (t_first < t_end) fetch(t_last);
-  for (int t0 = t_last; t0 >= t_first; t0 -= TT) {
-    const int steps = min(TT, t_end - t0);
-    if (loader) {
-      const int t = t0 + row, v = t < t_end ? valid : 0;
-      const float4 r4 = rd.get(pd + t * p.delta.sl, p.delta.vec, v), y4 = ry.get(py + t * p.dy.sl, p.dy.vec, v);
-      float4 z4 = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (gate) z4 = rz.get(pz + t * p.z.sl, p.z.vec, v);
-      const float rs[4] = {r4.x, r4.y, r4.z, r4.w}, gs[4] = {y4.x, y4.y, y4.z, y4.w}, zs[4] = {z4.x, z4.y, z4.z, z4.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = rs[i] + bias[i], g = gate ? gs[i] * zs[i] * sigmoid(zs[i]) : gs[i];
-        float dl = p.softplus ? softplus(x) : x;
-        dl = i < v ? dl : 0.f;
-        dg[row][col + i] = make_float4(dl, dl, g, g);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int id = tid + i * Sh::NT, r = id / (S / 4), c = id % (S / 4) * 4;
-      if (r < TT && t0 + r < t_end) *reinterpret_cast<float4*>(&cs[r][c]) = rc[i].get(pc + (t0 + r) * p.C.sl + c, p.C.vec, 4);
-    }
-    const unsigned resets = reset_bits(p, at.n, t0, steps);
+  unsigned resets = 0u;
+  if (t_first < t_end) {
+    stage(0);
+    resets = reset_bits(p, at.n, t_last, t_end - t_last);
+    if (t_last - TT >= t_first) fetch(t_last - TT);
     __syncthreads();
-    if (t0 - TT >= t_first) fetch(t0 - TT);
-#pragma unroll 4
-    for (int t = steps - 1; t >= 0; --t) {
-      const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&dg[t][chl]);
-      u64 c2[NP];
-      load_states<Sh>(&cs[t][0], q, c2);
-      const bool fresh = resets >> t & 1u;
-      cut |= fresh;
-      sum_d += dg[t][chl].x;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const u64 g = fma2<true>(c2[i], x.y, gc[i]), a = exp2_pair(mul2(x.x, A2[i]));
-        gc[i] = fresh ? 0ull : mul2(a, g);
-      }
+  }
+  for (int t0 = t_last, k0 = 0; t0 >= t_first; t0 -= TT, k0 ^= 1) {
+    const int steps = min(TT, t_end - t0);
+    const unsigned now = resets;
+    if (t0 - TT >= t_first) {
+      stage(k0 ^ 1);
+      resets = reset_bits(p, at.n, t0 - TT, TT);
+      if (t0 - 2 * TT >= t_first) fetch(t0 - 2 * TT);
     }
+    auto walk = [&](auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+#pragma unroll
+      for (int t = TT - 1; t >= 0; --t) {
+        if (!WHOLE && t >= steps) continue;
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&dg[k0][t][here]);
+        u64 c2[NP];
+        load_states<Sh>(&cs[k0][t][0], q, c2);
+        const bool fresh = !WHOLE && (now >> t & 1u);
+        cut |= fresh;
+        sum_d += __uint_as_float((unsigned)x.x);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const u64 g = fma2<true>(c2[i], x.y, gc[i]), a = exp2_pair(mul2(x.x, A2[i]));
+          gc[i] = fresh ? 0ull : mul2(a, g);
+        }
+      }
+    };
+    if (steps == TT && now == 0u) walk(std::true_type());
+    else walk(std::false_type());
     __syncthreads();
   }
   if (!mine) return;
@@ -420,7 +508,8 @@ __global__ void __launch_bounds__(256) scan_sums_kernel(const ScanParams p, int 
     const int e = (int)(k - r * GS), g = e / p.S, s = e - g * p.S;
     const ScanRows& o = second ? p.dC : p.dB;
     T* dst = reinterpret_cast<T*>(o.p) + r / p.L * o.sn + r % p.L * o.sl + g * o.sg + s;
-    put4(dst, o.vec, 4, v);
+    if (p.vec) put4<true>(dst, 4, v);
+    else put4<false>(dst, 4, v);
     return;
   }
   const long long i = (long long)(blockIdx.x - bc_blocks) * 256 + threadIdx.x, na = (long long)p.D * p.S;
@@ -436,9 +525,9 @@ __global__ void __launch_bounds__(256) scan_sums_kernel(const ScanParams p, int 
   else if (p.dbias) p.dbias[i - na - p.D] = v;
 }
 
-template <typename T, int S>
+template <typename T, int S, bool VEC>
 cudaError_t launch(const ScanParams& p, cudaStream_t s) {
-  const unsigned grid = (unsigned)(blocks_of<S>(p) * p.N);
+  const unsigned grid = (unsigned)(blocks_of(p) * p.N);
   constexpr int smem = sizeof(BwdSmem<S>);
   static unsigned long long raised = 0;      // devices whose limit is raised
   if (smem > 48 * 1024) {
@@ -446,32 +535,22 @@ cudaError_t launch(const ScanParams& p, cudaStream_t s) {
     if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(__atomic_load_n(&raised, __ATOMIC_ACQUIRE) & bit)) {
-      const cudaError_t e = cudaFuncSetAttribute(scan_bwd_kernel<T, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      const cudaError_t e = cudaFuncSetAttribute(scan_bwd_kernel<T, S, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       if (e != cudaSuccess) return e;
       __atomic_fetch_or(&raised, bit, __ATOMIC_RELEASE);
     }
   }
   if (p.nseg > 1) {
-    scan_bwd_carry_kernel<T, S><<<dim3(grid, p.nseg - 1), Shape<S>::NT, 0, s>>>(p);
+    scan_bwd_carry_kernel<T, S, VEC><<<dim3(grid, p.nseg - 1), Shape<S>::NT, 0, s>>>(p);
     if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   }
-  scan_bwd_kernel<T, S><<<dim3(grid, p.nseg), Shape<S>::NT, smem, s>>>(p);
+  scan_bwd_kernel<T, S, VEC><<<dim3(grid, p.nseg), Shape<S>::NT, smem, s>>>(p);
   if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   const long long quads = 2ll * p.N * p.L * p.G * S / 4, bc_blocks = (quads + 255) / 256;
   const long long rest = ((long long)p.D * S + 2 * p.D + 255) / 256;
   scan_sums_kernel<T><<<(unsigned)(bc_blocks + rest), 256, 0, s>>>(p, (int)bc_blocks);
   return cudaGetLastError();
 }
-template <typename T>
-cudaError_t by_states(const ScanParams& p, cudaStream_t s) {
-  switch (p.S) {
-    case 8: return launch<T, 8>(p, s);
-    case 16: return launch<T, 16>(p, s);
-    case 32: return launch<T, 32>(p, s);
-    default: return launch<T, 64>(p, s);
-  }
-}
-
 }  // namespace
 
 int scan_bwd_segments(int N, int L, int D, int sms) { return scan_segments(N, L, D, sms); }
@@ -489,7 +568,7 @@ long long scan_bwd_scratch(ScanParams& p, float* base) {
   return bc + a + v + carry;
 }
 cudaError_t scan_backward(const ScanParams& p, cudaStream_t s) {
-  return p.bf16 ? by_states<__nv_bfloat16>(p, s) : by_states<float>(p, s);
+  return by_shape(p, [&](auto t, auto states, auto vec) { return launch<decltype(t), decltype(states)::value, decltype(vec)::value>(p, s); });
 }
 
 }  // namespace srwm

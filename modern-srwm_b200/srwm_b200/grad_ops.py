@@ -21,7 +21,7 @@ def grad_norm(tensors):
     tensors = [t.detach() for t in tensors]
     if not tensors:
         return torch.zeros(())
-    r = L.host().grads_norm(tensors, -1.0)
+    r = L.host().grads_norm(tensors, -1.0, False)
     return _checked(tensors, -1.0) if r is NotImplemented else r
 
 
@@ -29,6 +29,11 @@ def grad_norm(tensors):
 def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     if isinstance(parameters, torch.Tensor):
         parameters = (parameters,)
+    parameters = list(parameters)
+    if not error_if_nonfinite and 0.0 <= float(max_norm):
+        r = L.host().grads_norm(parameters, float(max_norm), True)
+        if r is not NotImplemented:
+            return r
     grads = [p.grad for p in parameters if p.grad is not None]
     return clip_tensors_(grads, max_norm, error_if_nonfinite)
 
@@ -43,7 +48,7 @@ def clip_tensors_(grads, max_norm, error_if_nonfinite=False):
         return torch.zeros(())
     if error_if_nonfinite and not torch.isfinite(norm := grad_norm(grads)):
         raise RuntimeError(f"the norm of the gradients is not finite ({float(norm)}); they have not been scaled")
-    r = L.host().grads_norm(grads, max_norm)
+    r = L.host().grads_norm(grads, max_norm, False)
     return _checked(grads, max_norm) if r is NotImplemented else r
 
 
@@ -61,7 +66,7 @@ def _checked(tensors, max_norm):
             raise TypeError("gradients must be dense tensors")
     plain = [t.detach().as_subclass(torch.Tensor) for t in tensors]
     dense = [t.contiguous() for t in plain]      # (the same memory where it is dense already)
-    r = L.host().grads_norm(dense, max_norm)
+    r = L.host().grads_norm(dense, max_norm, False)
     if r is NotImplemented:
         raise ValueError("gradients overlap in memory (the same one twice, or views of one another)")
     if max_norm >= 0.0:
