@@ -934,7 +934,7 @@ static bool off(const void* p, int es) { return (uintptr_t)p % es != 0; }
 static int scan_sizes(int64_t N, int64_t L, int64_t D, int64_t S, int64_t G) {
   if (N < 0 || L < 0 || D < 0 || G <= 0 || D % G) return SRWM_B200_ERR_SHAPE;
   if (!head_dim_ok((int)S)) return SRWM_B200_ERR_HEAD_DIM;
-  const int64_t blocks = (D / G + srwm::SCAN_CH - 1) / srwm::SCAN_CH * G;
+  const int64_t blocks = (D / G + 31) / 32 * G;
   // one CTA per sequence and 32 channels; four values of dB or dC per thread of the sums' kernel
   if (blocks * N > 0x7fffffffLL || N * L > 0x7fffffffLL || N * L * G * S / 2 / 256 > 0x7f000000LL) return SRWM_B200_ERR_SHAPE;
   return 0;

@@ -5,8 +5,8 @@
 // for each channel with S states of its own; B and C are common to a group's channels.  Per state and step that is one
 // exponential and four fp32 operations: with 16 exponentials and 128 fp32 operations a cycle and multiprocessor, the exponentials
 // bind (the streams are 8 bytes a channel and step in bf16, read and written in less time than 16 states' exponentials take).  So a thread holds some
-// states of one channel in registers and walks the time axis; LN neighbouring lanes share a channel.  What belongs to a channel and
-// step (softplus, the gate) is formed once per tile of 16 steps x 32 channels, by the thread that loads it.
+// states of one or two channels in registers and walks the time axis; LN neighbouring lanes share a channel.  What belongs to a channel and
+// step (softplus, the gate) is formed once per tile of 16 steps x 32 or 64 channels, by the thread that loads it.
 #pragma once
 #include <type_traits>
 
@@ -16,17 +16,22 @@
 namespace srwm {
 namespace scan {
 
-template <int S_>
+// C: neighbouring channels of a thread.  A step's B and C are then read once for C channels: with one, the shared-memory pipe (a 16-byte load
+// is four of its cycles) is busier than the exponentials' one.
+template <int S_, int C_>
 struct Shape {
-  static constexpr int S = S_;
-  static constexpr int LN = S == 64 ? 8 : 4;    // lanes of a channel
-  static constexpr int ST = S / LN;             // states of a thread (2, 4 or 8)
-  static constexpr int LC = 32 / LN;            // channels of a warp
-  static constexpr int NT = SCAN_CH * LN;       // threads
-  static constexpr int QUADS = 2 * SCAN_TILE * S / 4;
-  static constexpr int NQ = (QUADS + NT - 1) / NT;   // pieces of four of B and C that a thread loads
+  static constexpr int S = S_, C = C_;
+  static constexpr int LN = S == 8 ? 2 : S == 64 ? 8 : 4;    // lanes of a channel
+  static constexpr int ST = S / LN;                           // states of a thread and channel (4 or 8)
+  static constexpr int NP = ST / 2;                           // pairs of them
+  static constexpr int LC = 32 / LN;                          // channel groups of a warp
+  static constexpr int WARPS = LN < 4 ? 4 : LN, WALK = 32 * WARPS;      // warps and threads that walk the time axis
+  static constexpr int LOAD = 128, NT = WALK + LOAD;          // threads that load, prepare and write tiles beside them; all
+  static constexpr int CH = WARPS * LC * C;                   // channels of a CTA
+  static constexpr int PIECES = SCAN_TILE * CH / 4, NL = PIECES / LOAD;               // pieces of four channels of a tile; of a loading thread
+  static constexpr int QUADS = SCAN_TILE * S / 4, NQ = (QUADS + LOAD - 1) / LOAD;     // pieces of four of B (and of C)
   // state j of lane q: whole pieces of four lie side by side over the lanes, so that a warp reads B and C without conflicts
-  static __device__ __forceinline__ int first(int q, int piece) { return ST >= 4 ? piece * 4 * LN + q * 4 : q * ST; }
+  static __device__ __forceinline__ int first(int q, int piece) { return piece * 4 * LN + q * 4; }
 };
 
 __device__ __forceinline__ u64 mul2(u64 a, u64 b) {
@@ -142,13 +147,9 @@ __device__ __forceinline__ void put4(__nv_bfloat16* p, int valid, float4 v) {
   }
 }
 
-// Where a channel's value lies in a staged row of 16-byte pieces: a thread writes four neighbouring channels, a warp reads eight;
-// turned by one per eight channels both are free of conflicts
-__device__ __forceinline__ int swizzled(int ch) { return (ch & ~7) | ((ch + (ch >> 3)) & 7); }
-
 // Sums over a channel's LN lanes of LN steps' values: lane q gets step q's
 template <int LN>
-__device__ __forceinline__ float steps_to_lanes(float (&v)[LN], int q) {
+__device__ __forceinline__ float steps_to_lanes(float* v, int q) {
 #pragma unroll
   for (int w = 1; w < LN; w *= 2) {
     const bool up = q & w;
@@ -161,27 +162,30 @@ __device__ __forceinline__ float steps_to_lanes(float (&v)[LN], int q) {
   return v[0];
 }
 
-// A thread's states as pairs, from or to [S] floats of its channel
+// A thread's states of a channel as pairs, from or to that channel's [S] floats
 template <typename Sh>
-__device__ __forceinline__ void load_states(const float* p, int q, u64 (&v)[Sh::ST / 2]) {
-  if constexpr (Sh::ST >= 4) {
+__device__ __forceinline__ void load_states(const float* p, int q, u64* v) {
 #pragma unroll
-    for (int i = 0; i < Sh::ST / 4; ++i) {
-      const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(p + Sh::first(q, i));
-      v[2 * i] = t.x; v[2 * i + 1] = t.y;
-    }
-  } else {
-    v[0] = *reinterpret_cast<const u64*>(p + Sh::first(q, 0));
+  for (int i = 0; i < Sh::ST / 4; ++i) {
+    const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(p + Sh::first(q, i));
+    v[2 * i] = t.x; v[2 * i + 1] = t.y;
   }
 }
 template <typename Sh>
-__device__ __forceinline__ void store_states(float* p, int q, const u64 (&v)[Sh::ST / 2]) {
-  if constexpr (Sh::ST >= 4) {
+__device__ __forceinline__ void store_states(float* p, int q, const u64* v) {
 #pragma unroll
-    for (int i = 0; i < Sh::ST / 4; ++i)
-      *reinterpret_cast<ulonglong2*>(p + Sh::first(q, i)) = make_ulonglong2(v[2 * i], v[2 * i + 1]);
+  for (int i = 0; i < Sh::ST / 4; ++i)
+    *reinterpret_cast<ulonglong2*>(p + Sh::first(q, i)) = make_ulonglong2(v[2 * i], v[2 * i + 1]);
+}
+// C neighbouring values of a staged row
+template <int C>
+__device__ __forceinline__ void load_channels(const float2* p, float2* v) {
+  if constexpr (C == 2) {
+    const float4 t = *reinterpret_cast<const float4*>(p);
+    v[0] = make_float2(t.x, t.y);
+    v[1] = make_float2(t.z, t.w);
   } else {
-    *reinterpret_cast<u64*>(p + Sh::first(q, 0)) = v[0];
+    v[0] = *p;
   }
 }
 
@@ -192,15 +196,17 @@ __device__ __forceinline__ u64 exp2_pair(u64 x) {
   return pack2(ex2(a), ex2(b));
 }
 
-// Where a CTA works: sequence, group, first channel in the group
+// Where a CTA works: sequence, group, first channel, channels of the group from there on
+template <int CH>
 struct Place {
-  int n, g, ch0, left;      // left: channels of the group from ch0 on
+  int n, g, ch0, left, blk;
   __device__ __forceinline__ Place(const ScanParams& p, int index) {
-    const int Dg = p.D / p.G, per = (Dg + SCAN_CH - 1) / SCAN_CH, blocks = per * p.G;
+    const int Dg = p.D / p.G, per = (Dg + CH - 1) / CH, blocks = per * p.G;
     n = index / blocks;
     const int b = index - n * blocks;
     g = b / per;
-    ch0 = (b - g * per) * SCAN_CH;
+    blk = b - g * per;
+    ch0 = blk * CH;
     left = Dg - ch0;
     ch0 += g * Dg;
   }
@@ -214,9 +220,9 @@ __device__ __forceinline__ unsigned reset_bits(const ScanParams& p, int n, int t
   return __ballot_sync(0xffffffffu, r);
 }
 
-inline int blocks_of(const ScanParams& p) {
+inline long long blocks_of(const ScanParams& p, int channels) {
   const int Dg = p.D / p.G;
-  return (Dg + SCAN_CH - 1) / SCAN_CH * p.G;
+  return (long long)((Dg + channels - 1) / channels) * p.G * p.N;
 }
 
 // f(element, states, vec) as types

@@ -7,7 +7,6 @@ namespace srwm {
 
 constexpr int SCAN_CKPT = 8;    // steps between the states that a training forward keeps
 constexpr int SCAN_TILE = 16;   // steps that a CTA stages at a time
-constexpr int SCAN_CH = 32;     // channels of a CTA
 constexpr int SCAN_STEPS_DIRECT = 4;   // up to so many steps without gradients take the kernel of single tokens
 
 struct ScanRows {               // [N, L, D] (or [N, L, G, S]), innermost dense; strides in elements
@@ -34,6 +33,7 @@ struct ScanParams {
   float *part_bc, *part_a, *part_v;
 };
 
+__host__ __device__ constexpr int scan_bwd_channels(int S) { return S == 8 ? 128 : S == 16 ? 64 : 32; }      // of a CTA of the backward
 int scan_segments(int N, int L, int D, int sms);          // pieces that a call's time axis is cut into
 int scan_bwd_segments(int N, int L, int D, int sms);
 long long scan_fwd_scratch(const ScanParams& p);           // floats

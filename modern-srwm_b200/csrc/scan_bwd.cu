@@ -3,9 +3,8 @@
 // With g_t = dL/dh_t = C_t dy'_t + a_{t+1} g_{t+1} (dy' = dy silu(z), a = exp(Delta A)):
 //   dC_t = sum_d dy'_t h_t        dB_t = sum_d g_t Delta_t u_t        dA = sum_t Delta_t g_t a_t h_{t-1}
 //   du_t = D dy'_t + Delta_t (g_t . B_t)        dDelta_t = u_t (g_t . B_t) + sum_s A a_t h_{t-1} g_t
-// A CTA takes its 32 channels from the last step to the first.  The states in front of each eighth step are the forward's; within
-// eight steps they are formed again, a_t and a_t h_{t-1} staying in registers until the way back has used them (four steps of them
-// where a thread has eight states: the first four are walked twice then).  Thirteen fp32
+// A CTA takes its 64 (32) channels from the last step to the first.  The states in front of each eighth step are the forward's; within
+// eight steps they are formed again, four at a time, a_t and a_t h_{t-1} staying in registers until the way back has used them.  Thirteen fp32
 // operations per state and step bind.  Sums over states go through a channel's lanes, sums over channels (dB, dC) through the
 // warp's other lanes and shared memory, and are added up over the CTAs by a second launch, in a fixed order.
 #include <type_traits>
@@ -17,12 +16,14 @@ namespace srwm {
 namespace {
 using namespace scan;
 
-// Sums of eight values over a warp's LC channels: 8 / LC values stay with each lane, those from index `kept_of` on
-template <int LN, int LC>
-__device__ __forceinline__ void channels_to_lanes(float (&v)[8], int lane) {
+// Sums of eight values over a warp's 32 / LN channel groups: 8 values (or one, where there are eight groups or more) stay with each
+// lane, those from index kept_of on
+template <int LN>
+__device__ __forceinline__ void groups_to_lanes(float* v, int lane) {
 #pragma unroll
   for (int w = LN, half = 4; w < 32; w *= 2, half /= 2) {
     const bool up = lane & w;
+    if (half == 0) v[0] += __shfl_xor_sync(0xffffffffu, v[0], w);
 #pragma unroll
     for (int i = 0; i < half; ++i) {
       const float keep = up ? v[half + i] : v[i], send = up ? v[i] : v[half + i];
@@ -30,449 +31,584 @@ __device__ __forceinline__ void channels_to_lanes(float (&v)[8], int lane) {
     }
   }
 }
-template <int LN, int LC>
+template <int LN>
 __device__ __forceinline__ int kept_of(int lane) {
-  const int c = lane / LN;       // bits of the channel, the lowest first halves
-  return LC == 8 ? (c & 1) * 4 + (c & 2) + (c >> 2) : (c & 1) * 4 + (c & 2);
+  const int c = lane / LN;       // the lowest bit of the group halves first
+  return LN == 8 ? (c & 1) * 4 + (c & 2) : (c & 1) * 4 + (c & 2) + (c >> 2 & 1);
 }
 
+// Two channels a thread with up to 16 states, one with more: eight states of a thread in all
+template <int S>
+using BwdShape = Shape<S, S <= 16 ? 2 : 1>;
+
+// Two buffers: a tile is loaded and prepared, and the results of the one before it written, while the tile between is walked
 template <int S>
 struct BwdSmem {
-  static constexpr int TT = SCAN_TILE, CH = SCAN_CH, PAD = CH + 8, WARPS = Shape<S>::NT / 32;
-  float4 dd[TT][CH];           // Delta twice, Delta u twice
-  float2 gy[TT][CH];           // dy' twice
-  float bc[2][TT][S];
-  float gb[TT][PAD], sa[TT][PAD], yp[TT][PAD];
-  float part[WARPS][TT][2][S];
+  using Sh = BwdShape<S>;
+  static constexpr int TT = SCAN_TILE, CH = Sh::CH, PAD = CH + 8;
+  struct Tile {
+    float2 dd[TT][CH];           // Delta, Delta u
+    float gy[TT][CH];            // dy'
+    float bc[2][TT][S];
+    float gb[TT][PAD], sa[TT][PAD], yp[TT][PAD];
+    float part[Sh::WARPS][TT][2][S];
+  } tile[2];
+  float4 sums[2][Sh::PIECES];    // of dy' u and of the gradient of delta, a slot for each loading thread's piece
 };
 
-// Steps whose a and a h stay in registers, and CTAs that a multiprocessor is to hold (168 registers a thread, or 128)
-template <int S>
-struct BwdPlan {
-  static constexpr int SUB = Shape<S>::ST == 8 ? 4 : 8, CTAS = S == 8 ? 4 : S == 64 ? 1 : 2;
+// Registers: the walking threads' share and the loading threads', which together are what the CTA is launched with (128 a thread, two CTAs
+// a multiprocessor; S 64: 168 and one)
+template <typename T, int S>
+struct BwdRegs {
+  static constexpr int CTAS = S == 64 ? 1 : 2, LOADERS = 104;
+  static constexpr int WALKERS = S == 64 ? 200 : 256 - LOADERS;
 };
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <typename T, int S, bool VEC>
-__global__ void __launch_bounds__(Shape<S>::NT, BwdPlan<S>::CTAS) scan_bwd_kernel(const ScanParams p) {
-  using Sh = Shape<S>;
-  constexpr int TT = SCAN_TILE, CH = SCAN_CH, KT = SCAN_CKPT, NP = Sh::ST / 2, GS = 8 / Sh::ST, KEPT = 8 / Sh::LC, SUB = BwdPlan<S>::SUB;
-  constexpr int WARPS = BwdSmem<S>::WARPS;
-  extern __shared__ __align__(16) unsigned char raw_smem[];
-  BwdSmem<S>& sm = *reinterpret_cast<BwdSmem<S>*>(raw_smem);
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, q = lane % Sh::LN, chl = warp * Sh::LC + lane / Sh::LN;
-  const Place at(p, blockIdx.x);
+__device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& sm) {
+  using Sh = BwdShape<S>;
+  constexpr int TT = SCAN_TILE, CH = Sh::CH, NL = Sh::NL, NQ = Sh::NQ;
+  const int tid = threadIdx.x - Sh::WALK;
+  const Place<CH> at(p, blockIdx.x);
   const int seg = blockIdx.y, t_first = seg * p.seglen, t_end = min(p.L, t_first + p.seglen);
   const int t_last = t_first + (t_end - t_first - 1) / TT * TT;
-  const bool mine = chl < at.left;
-  const int d = at.ch0 + chl, here = swizzled(chl);
-
-  const bool loader = tid < TT * CH / 4;
-  const int row = tid / (CH / 4), col = tid % (CH / 4) * 4, valid = loader ? max(0, min(4, at.left - col)) : 0;
-  auto rows = [&](const ScanRows& w) { return reinterpret_cast<T*>(w.p) + at.n * w.sn + (t_last + row) * w.sl + at.ch0 + col; };
-  const T *pu = rows(p.u), *pd = rows(p.delta), *pz = rows(p.z), *py = rows(p.dy);
-  T *ou = rows(p.du), *od = rows(p.ddelta), *oz = rows(p.dz);
   const bool gate = p.z.p != nullptr;
-  float bias[4], skip[4], sum_skip[4], sum_bias[4];
+  // piece k: row (tid + k LOAD) / (CH / 4), columns from (tid % (CH / 4)) * 4 on
+  static_assert(Sh::LOAD % (CH / 4) == 0, "all pieces of a thread have the same columns");
+  constexpr int RS = Sh::LOAD / (CH / 4);       // rows between a thread's pieces
+  const int row = tid / (CH / 4), col = tid % (CH / 4) * 4, valid = max(0, min(4, at.left - col));
+#pragma unroll
+  for (int k = 0; k < NL; ++k) sm.sums[0][tid + k * Sh::LOAD] = sm.sums[1][tid + k * Sh::LOAD] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto place = [&](const ScanRows& w, int t) { return reinterpret_cast<T*>(w.p) + at.n * w.sn + t * w.sl + at.ch0 + col; };
+  float bias[4], skip[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     bias[i] = i < valid && p.bias ? p.bias[at.ch0 + col + i] : 0.f;
     skip[i] = i < valid && p.skip ? p.skip[at.ch0 + col + i] : 0.f;
-    sum_skip[i] = sum_bias[i] = 0.f;
   }
-  const T* pbc[Sh::NQ];
-  long long lbc[Sh::NQ];
-  int rbc[Sh::NQ];
+  Quad<T, VEC> fu[NL], fd[NL], fz[NL], fy[NL], fb[NQ], fc[NQ];
+  auto fetch_rows = [&](int t0) {
 #pragma unroll
-  for (int i = 0; i < Sh::NQ; ++i) {
-    const int id = tid + i * Sh::NT, c = id % (S / 4) * 4, r = id / (S / 4) % TT;
-    const bool second = id >= TT * S / 4;
-    lbc[i] = (second ? p.C.sl : p.B.sl) * TT;
-    pbc[i] = second ? reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + (t_last + r) * p.C.sl + c
-                    : reinterpret_cast<const T*>(p.B.p) + at.n * p.B.sn + at.g * p.B.sg + (t_last + r) * p.B.sl + c;
-    rbc[i] = id < Sh::QUADS ? r : p.L;
-  }
-  Quad<T, VEC> fu, fd, fz, fy, fbc[Sh::NQ];
-  auto fetch = [&](int t0) {      // tiles are asked for in order, the last first
-    const int v = t0 + row < t_end ? valid : 0;
-    fu.fetch(pu, v);
-    fd.fetch(pd, v);
-    fy.fetch(py, v);
-    if (gate) fz.fetch(pz, v);
-    pu -= TT * p.u.sl; pd -= TT * p.delta.sl; py -= TT * p.dy.sl; pz -= TT * p.z.sl;
-#pragma unroll
-    for (int i = 0; i < Sh::NQ; ++i) {
-      fbc[i].fetch(pbc[i], t0 + rbc[i] < t_end ? 4 : 0);
-      pbc[i] -= lbc[i];
+    for (int k = 0; k < NL; ++k) {
+      const int t = t0 + row + k * RS, v = t < t_end ? valid : 0;
+      fu[k].fetch(place(p.u, t), v);
+      fd[k].fetch(place(p.delta, t), v);
+      fy[k].fetch(place(p.dy, t), v);
+      if (gate) fz[k].fetch(place(p.z, t), v);
     }
   };
-
-  u64 A2[NP], gc[NP], dA[NP];
+  auto fetch_bc = [&](int t0) {
 #pragma unroll
-  for (int i = 0; i < NP; ++i) A2[i] = gc[i] = dA[i] = 0ull;
-  if (t_first < t_end) fetch(t_last);
-  const long long states = (long long)p.N * p.D * S, own = ((long long)at.n * p.D + d) * S;
-  const int nck = (p.L + KT - 1) / KT;
-  if (mine) {
-    load_states<Sh>(p.A + (long long)d * S, q, A2);
-    const u64 l2 = dup2(LOG2E);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) A2[i] = mul2(A2[i], l2);
-    if (p.dhT) load_states<Sh>(p.dhT + own, q, gc);
-#pragma unroll 4
-    for (int i = p.nseg - 1; i > seg; --i) {      // the pieces behind, the last first
-      u64 decay[NP], end[NP];
-      load_states<Sh>(p.carry + (2 * i - 2) * states + own, q, end);
-      load_states<Sh>(p.carry + (2 * i - 1) * states + own, q, decay);
-#pragma unroll
-      for (int k = 0; k < NP; ++k) gc[k] = fma2<true>(decay[k], gc[k], end[k]);
+    for (int i = 0; i < NQ; ++i) {
+      const int id = tid + i * Sh::LOAD, c = id % (S / 4) * 4, t = t0 + id / (S / 4), v = id < Sh::QUADS && t < t_end ? 4 : 0;
+      fb[i].fetch(reinterpret_cast<const T*>(p.B.p) + at.n * p.B.sn + at.g * p.B.sg + t * p.B.sl + c, v);
+      fc[i].fetch(reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + t * p.C.sl + c, v);
     }
-  }
-  const int kept = kept_of<Sh::LN, Sh::LC>(lane), kept_step = kept / Sh::ST, kept_j = kept % Sh::ST;
-  const int kept_state = Sh::first(q, kept_j / 4) + (Sh::ST >= 4 ? kept_j % 4 : kept_j);
-  float* part_mine = &sm.part[warp][kept_step][0][kept_state];
-
-  for (int t0 = t_last; t0 >= t_first; t0 -= TT) {
-    const int steps = min(TT, t_end - t0);
-    // the states in front of the tile's two halves
-    u64 ck[2][NP];
+  };
+  auto stage = [&](int buf) {
+    auto& tl = sm.tile[buf];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int i = 0; i < NP; ++i) ck[k][i] = 0ull;
-      if (mine && k * KT < steps) load_states<Sh>(p.ckpt + (((long long)at.n * nck + t0 / KT + k) * p.D + d) * S, q, ck[k]);
-    }
-    const Quad<T, VEC> qu = fu, qd = fd, qz = fz, qy = fy;
-    u64 dl2[2], g2v[2];      // Delta and dy' of this thread's piece
-    dl2[0] = dl2[1] = g2v[0] = g2v[1] = 0ull;
-    if (loader) {
-      const float4 u4 = qu.get(), r4 = qd.get(), y4 = qy.get();
-      dl2[0] = add2(pack2(r4.x, r4.y), pack2(bias[0], bias[1]));
-      dl2[1] = add2(pack2(r4.z, r4.w), pack2(bias[2], bias[3]));
+    for (int k = 0; k < NL; ++k) {
+      const float4 u4 = fu[k].get(), r4 = fd[k].get();
+      u64 lo = add2(pack2(r4.x, r4.y), pack2(bias[0], bias[1])), hi = add2(pack2(r4.z, r4.w), pack2(bias[2], bias[3]));
       if (p.softplus) {
-        dl2[0] = softplus2(dl2[0]);
-        dl2[1] = softplus2(dl2[1]);
+        lo = softplus2(lo);
+        hi = softplus2(hi);
       }
-      const u64 xlo = mul2(dl2[0], pack2(u4.x, u4.y)), xhi = mul2(dl2[1], pack2(u4.z, u4.w));
-      float dl[4], du[4], g[4] = {y4.x, y4.y, y4.z, y4.w};
-      unpack2(dl2[0], dl[0], dl[1]); unpack2(dl2[1], dl[2], dl[3]);
+      const u64 xlo = mul2(lo, pack2(u4.x, u4.y)), xhi = mul2(hi, pack2(u4.z, u4.w));
+      float dl[4], du[4];
+      float4 g = fy[k].get();
+      unpack2(lo, dl[0], dl[1]); unpack2(hi, dl[2], dl[3]);
       unpack2(xlo, du[0], du[1]); unpack2(xhi, du[2], du[3]);
       if (gate) {
-        const float4 z4 = qz.get();
-        g[0] *= z4.x * sigmoid(z4.x); g[1] *= z4.y * sigmoid(z4.y); g[2] *= z4.z * sigmoid(z4.z); g[3] *= z4.w * sigmoid(z4.w);
+        const float4 z4 = fz[k].get();
+        g.x *= z4.x * sigmoid(z4.x); g.y *= z4.y * sigmoid(z4.y); g.z *= z4.z * sigmoid(z4.z); g.w *= z4.w * sigmoid(z4.w);
       }
-      g2v[0] = pack2(g[0], g[1]); g2v[1] = pack2(g[2], g[3]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sm.dd[row][swizzled(col + i)] = make_float4(dl[i], dl[i], du[i], du[i]);
-        sm.gy[row][swizzled(col + i)] = make_float2(g[i], g[i]);
-      }
+      float4* o = reinterpret_cast<float4*>(&tl.dd[row + k * RS][col]);
+      o[0] = make_float4(dl[0], du[0], dl[1], du[1]);
+      o[1] = make_float4(dl[2], du[2], dl[3], du[3]);
+      *reinterpret_cast<float4*>(&tl.gy[row + k * RS][col]) = g;
     }
 #pragma unroll
-    for (int i = 0; i < Sh::NQ; ++i) {
-      const int id = tid + i * Sh::NT;
-      if (id < Sh::QUADS) *reinterpret_cast<float4*>(&sm.bc[0][0][0] + id * 4) = fbc[i].get();
+    for (int i = 0; i < NQ; ++i) {
+      const int id = tid + i * Sh::LOAD;
+      if (id >= Sh::QUADS) continue;
+      *reinterpret_cast<float4*>(&tl.bc[0][0][0] + id * 4) = fb[i].get();
+      *reinterpret_cast<float4*>(&tl.bc[1][0][0] + id * 4) = fc[i].get();
     }
-    const unsigned resets = reset_bits(p, at.n, t0, steps);
-    __syncthreads();
-    if (t0 - TT >= t_first) fetch(t0 - TT);
-
-    // SUB steps from s0 of the tile, h the state in front of them
-    auto steps_of = [&](auto whole, int s0, u64* h) __attribute__((always_inline)) {
-      constexpr bool WHOLE = decltype(whole)::value;
-      u64 a[SUB][NP], ah[SUB][NP];
-      float yv[Sh::LN], dc[8];
-#pragma unroll
-      for (int k = 0; k < SUB; ++k) {
-        const int t = s0 + k;
-        float* dck = dc + k % GS * Sh::ST;
-        yv[k % Sh::LN] = 0.f;
-#pragma unroll
-        for (int i = 0; i < Sh::ST; ++i) dck[i] = 0.f;
-        if (WHOLE || t < steps) {
-          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sm.dd[t][here]);
-          const u64 g2 = *reinterpret_cast<const u64*>(&sm.gy[t][here]);
-          const bool fresh = !WHOLE && (resets >> t & 1u);
-          u64 b2[NP], c2[NP], acc = 0ull;
-          load_states<Sh>(&sm.bc[0][t][0], q, b2);
-          load_states<Sh>(&sm.bc[1][t][0], q, c2);
-#pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            a[k][i] = exp2_pair(mul2(x.x, A2[i]));
-            if (fresh) a[k][i] = h[i] = 0ull;
-            ah[k][i] = mul2(a[k][i], h[i]);
-            h[i] = add2(ah[k][i], mul2(x.y, b2[i]));
-            acc = i == 0 ? mul2(h[i], c2[i]) : fma2<true>(h[i], c2[i], acc);
-            unpack2(mul2(h[i], g2), dck[2 * i], dck[2 * i + 1]);
-          }
-          yv[k % Sh::LN] = hsum2(acc);
-        }
-        if (k % GS == GS - 1) {
-          channels_to_lanes<Sh::LN, Sh::LC>(dc, lane);
-          float* o = part_mine + (s0 + k - (GS - 1)) * 2 * S + S;
-#pragma unroll
-          for (int i = 0; i < KEPT; ++i) o[i] = dc[i];
-        }
-        // (a piece's last steps may be fewer than the lanes: the values are zero then, and the row is not read)
-        if (gate && (k % Sh::LN == Sh::LN - 1 || k == SUB - 1)) {
-#pragma unroll
-          for (int i = SUB; i < Sh::LN; ++i) yv[i] = 0.f;
-          const float y = steps_to_lanes<Sh::LN>(yv, q);
-          if (SUB >= Sh::LN || q < SUB) sm.yp[s0 + k - (SUB < Sh::LN ? SUB : Sh::LN) + 1 + q][chl] = y;
-        }
-      }
-      float gbv[Sh::LN], sav[Sh::LN], db[8];
-#pragma unroll
-      for (int k = SUB - 1; k >= 0; --k) {
-        const int t = s0 + k;
-        float* dbk = db + k % GS * Sh::ST;
-        gbv[k % Sh::LN] = sav[k % Sh::LN] = 0.f;
-#pragma unroll
-        for (int i = 0; i < Sh::ST; ++i) dbk[i] = 0.f;
-        if (WHOLE || t < steps) {
-          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sm.dd[t][here]);
-          const u64 g2 = *reinterpret_cast<const u64*>(&sm.gy[t][here]);
-          u64 b2[NP], c2[NP], gb = 0ull, sa = 0ull;
-          load_states<Sh>(&sm.bc[0][t][0], q, b2);
-          load_states<Sh>(&sm.bc[1][t][0], q, c2);
-          const bool fresh = !WHOLE && (resets >> t & 1u);
-#pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            const u64 g = fma2<true>(c2[i], g2, gc[i]), gah = mul2(g, ah[k][i]);
-            gb = i == 0 ? mul2(g, b2[i]) : fma2<true>(g, b2[i], gb);
-            sa = i == 0 ? mul2(gah, A2[i]) : fma2<true>(gah, A2[i], sa);
-            dA[i] = fma2<true>(gah, x.x, dA[i]);
-            unpack2(mul2(g, x.y), dbk[2 * i], dbk[2 * i + 1]);
-            gc[i] = fresh ? 0ull : mul2(a[k][i], g);
-          }
-          gbv[k % Sh::LN] = hsum2(gb);
-          sav[k % Sh::LN] = hsum2(sa);
-        }
-        if (k % GS == 0) {
-          channels_to_lanes<Sh::LN, Sh::LC>(db, lane);
-          float* o = part_mine + (s0 + k) * 2 * S;
-#pragma unroll
-          for (int i = 0; i < KEPT; ++i) o[i] = db[i];
-        }
-        if (k % Sh::LN == 0) {
-#pragma unroll
-          for (int i = SUB; i < Sh::LN; ++i) gbv[i] = sav[i] = 0.f;
-          const float g = steps_to_lanes<Sh::LN>(gbv, q), s = steps_to_lanes<Sh::LN>(sav, q);
-          if (SUB >= Sh::LN || q < SUB) {
-            sm.gb[s0 + k + q][chl] = g;
-            sm.sa[s0 + k + q][chl] = s * 0.6931471805599453f;      // (A2 has log2(e) in it)
-          }
-        }
-      }
-    };
-    // eight steps at a time, the last first; where four stay in registers, the first four are walked on the way to the others
-    auto halves = [&](auto whole) {
-      constexpr bool WHOLE = decltype(whole)::value;
+  };
+  auto finish = [&](int t0, int buf) {
+    const auto& tl = sm.tile[buf];
+    const int steps = min(TT, t_end - t0);
+    // this CTA's share of dB and dC
 #pragma unroll 1
-      for (int s0 = TT - SUB; s0 >= 0; s0 -= SUB) {
-        if (!WHOLE && s0 >= steps) continue;
-        u64 h[NP];
+    for (int e = tid; e < steps * 2 * S / 4; e += Sh::LOAD) {
+      const int s = e % (S / 4) * 4, arr = e / (S / 4) % 2, t = e / (S / 2);
+      float4 v = *reinterpret_cast<const float4*>(&tl.part[0][t][arr][s]);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) h[i] = s0 >= KT ? ck[1][i] : ck[0][i];
-        if (SUB < KT && s0 % KT != 0) {
-#pragma unroll
-          for (int k = 0; k < SUB; ++k) {
-            const int t = s0 - SUB + k;
-            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sm.dd[t][here]);
-            u64 b2[NP];
-            load_states<Sh>(&sm.bc[0][t][0], q, b2);
-            const bool fresh = !WHOLE && (resets >> t & 1u);
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-              u64 a = exp2_pair(mul2(x.x, A2[i]));
-              if (fresh) a = h[i] = 0ull;
-              h[i] = add2(mul2(a, h[i]), mul2(x.y, b2[i]));
-            }
-          }
-        }
-        steps_of(whole, s0, h);
+      for (int w = 1; w < Sh::WARPS; ++w) {
+        const float4 o = *reinterpret_cast<const float4*>(&tl.part[w][t][arr][s]);
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
       }
-    };
-    if (steps == TT && resets == 0u) halves(std::true_type());
-    else halves(std::false_type());
-    __syncthreads();
-    {   // this CTA's share of dB and dC
-      const int per = ((p.D / p.G) + CH - 1) / CH, blk = (int)(blockIdx.x % (unsigned)per);
-#pragma unroll
-      for (int e = tid; e < TT * 2 * S / 4; e += Sh::NT) {
-        const int s = e % (S / 4) * 4, arr = e / (S / 4) % 2, t = e / (S / 2);
-        float4 v = *reinterpret_cast<const float4*>(&sm.part[0][t][arr][s]);
-#pragma unroll
-        for (int w = 1; w < WARPS; ++w) {
-          const float4 o = *reinterpret_cast<const float4*>(&sm.part[w][t][arr][s]);
-          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-        }
-        if (t < steps)
-          *reinterpret_cast<float4*>(p.part_bc + ((((long long)blk * 2 + arr) * p.N + at.n) * p.L + t0 + t) * p.G * S + at.g * S + s) = v;
-      }
+      *reinterpret_cast<float4*>(p.part_bc + ((((long long)at.blk * 2 + arr) * p.N + at.n) * p.L + t0 + t) * p.G * S + at.g * S + s) = v;
     }
-    const int v = row < steps ? valid : 0;
-    if (v > 0) {
-      const float4 gb4 = *reinterpret_cast<const float4*>(&sm.gb[row][col]), sa4 = *reinterpret_cast<const float4*>(&sm.sa[row][col]);
-      const float4 u4 = qu.get(), r4 = qd.get();
-      const float us[4] = {u4.x, u4.y, u4.z, u4.w}, rs[4] = {r4.x, r4.y, r4.z, r4.w};
-      const float gb[4] = {gb4.x, gb4.y, gb4.z, gb4.w}, sa[4] = {sa4.x, sa4.y, sa4.z, sa4.w};
-      float dl[4], g[4], o1[4], o2[4];
-      unpack2(dl2[0], dl[0], dl[1]); unpack2(dl2[1], dl[2], dl[3]);
-      unpack2(g2v[0], g[0], g[1]); unpack2(g2v[1], g[2], g[3]);
+    // (the tile's rows again: they have left the registers)
+#pragma unroll 1
+    for (int k = 0; k < NL; ++k) {
+      const int r = row + k * RS, t = t0 + r, v = r < steps ? valid : 0;
+      if (v <= 0) break;
+      Quad<T, VEC> q0, q1, q2, q3;
+      q0.fetch(place(p.u, t), v);
+      q1.fetch(place(p.delta, t), v);
+      if (gate) {
+        q2.fetch(place(p.z, t), v);
+        q3.fetch(place(p.dy, t), v);
+      }
+      const float4 gb4 = *reinterpret_cast<const float4*>(&tl.gb[r][col]), sa4 = *reinterpret_cast<const float4*>(&tl.sa[r][col]);
+      const float4 g4 = *reinterpret_cast<const float4*>(&tl.gy[r][col]);
+      const float4* dk = reinterpret_cast<const float4*>(&tl.dd[r][col]);
+      const float4 d01 = dk[0], d23 = dk[1], u4 = q0.get(), r4 = q1.get();
+      const float dl[4] = {d01.x, d01.z, d23.x, d23.z}, us[4] = {u4.x, u4.y, u4.z, u4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w};
+      const float rs[4] = {r4.x, r4.y, r4.z, r4.w}, gb[4] = {gb4.x, gb4.y, gb4.z, gb4.w}, sa[4] = {sa4.x, sa4.y, sa4.z, sa4.w};
+      float o1[4], o2[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         o1[i] = fmaf(g[i], skip[i], dl[i] * gb[i]);
         o2[i] = fmaf(us[i], gb[i], sa[i]);
         if (p.softplus) o2[i] *= sigmoid(rs[i] + bias[i]);
-        if (i < v) {
-          sum_skip[i] = fmaf(g[i], us[i], sum_skip[i]);
-          sum_bias[i] += o2[i];
-        }
       }
-      put4<VEC>(ou, v, make_float4(o1[0], o1[1], o1[2], o1[3]));
-      put4<VEC>(od, v, make_float4(o2[0], o2[1], o2[2], o2[3]));
+      put4<VEC>(place(p.du, t), v, make_float4(o1[0], o1[1], o1[2], o1[3]));
+      put4<VEC>(place(p.ddelta, t), v, make_float4(o2[0], o2[1], o2[2], o2[3]));
+      const int id = tid + k * Sh::LOAD;
+      float4 w = sm.sums[0][id];
+      sm.sums[0][id] = make_float4(fmaf(g[0], us[0], w.x), fmaf(g[1], us[1], w.y), fmaf(g[2], us[2], w.z), fmaf(g[3], us[3], w.w));
+      w = sm.sums[1][id];
+      sm.sums[1][id] = make_float4(w.x + o2[0], w.y + o2[1], w.z + o2[2], w.w + o2[3]);
       if (gate) {
-        const float4 yp4 = *reinterpret_cast<const float4*>(&sm.yp[row][col]), z4 = qz.get(), y4 = qy.get();
+        const float4 yp4 = *reinterpret_cast<const float4*>(&tl.yp[r][col]), z4 = q2.get(), y4 = q3.get();
         const float yp[4] = {yp4.x, yp4.y, yp4.z, yp4.w}, zs[4] = {z4.x, z4.y, z4.z, z4.w}, os[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float sg = sigmoid(zs[i]);
           o1[i] = os[i] * fmaf(skip[i], us[i], yp[i]) * sg * fmaf(zs[i], 1.f - sg, 1.f);
         }
-        put4<VEC>(oz, v, make_float4(o1[0], o1[1], o1[2], o1[3]));
+        put4<VEC>(place(p.dz, t), v, make_float4(o1[0], o1[1], o1[2], o1[3]));
       }
     }
-    ou -= TT * p.du.sl; od -= TT * p.ddelta.sl; oz -= TT * p.dz.sl;
-  }
-  const long long slot = (long long)at.n * p.nseg + seg;
-  if (mine) {
-    store_states<Sh>(p.part_a + (slot * p.D + d) * S, q, dA);
-    if (seg == 0 && p.dh0) store_states<Sh>(p.dh0 + own, q, gc);
+  };
+  fetch_rows(t_last);
+  fetch_bc(t_last);
+  stage(0);
+  if (t_last - TT >= t_first) {
+    fetch_rows(t_last - TT);
+    fetch_bc(t_last - TT);
   }
   __syncthreads();
-  if (loader) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sm.gb[row][col + i] = sum_skip[i];
-      sm.sa[row][col + i] = sum_bias[i];
+  int k0 = 0;
+  for (int t0 = t_last; t0 >= t_first; t0 -= TT, k0 ^= 1) {
+    if (t0 < t_last) finish(t0 + TT, k0 ^ 1);
+    if (t0 - TT >= t_first) {
+      stage(k0 ^ 1);
+      if (t0 - 2 * TT >= t_first) {
+        fetch_rows(t0 - 2 * TT);
+        fetch_bc(t0 - 2 * TT);
+      }
     }
+    __syncthreads();
   }
-  __syncthreads();
-  if (tid < 2 * CH) {
-    const int c = tid % CH, which = tid / CH;
+  finish(t_first, k0 ^ 1);
+  asm volatile("bar.sync 1, %0;" ::"n"(Sh::LOAD) : "memory");      // the loading threads alone
+  const long long slot = (long long)at.n * p.nseg + seg;
+  for (int e = tid; e < 2 * CH; e += Sh::LOAD) {
+    const int c = e % CH, which = e / CH;
+    const float* f = reinterpret_cast<const float*>(&sm.sums[which][0]) + c;
     float v = 0.f;
 #pragma unroll
-    for (int r = 0; r < TT; ++r) v += which ? sm.sa[r][c] : sm.gb[r][c];
+    for (int r = 0; r < TT; ++r) v += f[r * CH];
     if (c < at.left) p.part_v[(slot * 2 + which) * p.D + at.ch0 + c] = v;
+  }
+}
+
+template <typename T, int S, bool VEC>
+__device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& sm) {
+  using Sh = BwdShape<S>;
+  constexpr int TT = SCAN_TILE, CH = Sh::CH, KT = SCAN_CKPT, C = Sh::C, NP = Sh::NP, ST = Sh::ST, LN = Sh::LN;
+  constexpr int SUB = 4, GS = 8 / ST, KEPT = LN == 8 ? 2 : 1;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, q = lane % LN, chl = (warp * Sh::LC + lane / LN) * C;
+  const Place<CH> at(p, blockIdx.x);
+  const int seg = blockIdx.y, t_first = seg * p.seglen, t_end = min(p.L, t_first + p.seglen);
+  const int t_last = t_first + (t_end - t_first - 1) / TT * TT;
+  const int d = at.ch0 + chl, mine = at.left - chl;
+  const bool gate = p.z.p != nullptr;
+
+  u64 A2[C][NP], gc[C][NP], dA[C][NP];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < NP; ++i) A2[c][i] = gc[c][i] = dA[c][i] = 0ull;
+  const long long states = (long long)p.N * p.D * S, own = ((long long)at.n * p.D + d) * S;
+  const int nck = (p.L + KT - 1) / KT;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (c >= mine) continue;
+    load_states<Sh>(p.A + (long long)(d + c) * S, q, A2[c]);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) A2[c][i] = mul2(A2[c][i], dup2(LOG2E));
+    const long long o = own + c * S;
+    if (p.dhT) load_states<Sh>(p.dhT + o, q, gc[c]);
+#pragma unroll 4
+    for (int i = p.nseg - 1; i > seg; --i) {      // the pieces behind, the last first
+      u64 decay[NP], end[NP];
+      load_states<Sh>(p.carry + (2 * i - 2) * states + o, q, end);
+      load_states<Sh>(p.carry + (2 * i - 1) * states + o, q, decay);
+#pragma unroll
+      for (int k = 0; k < NP; ++k) gc[c][k] = fma2<true>(decay[k], gc[c][k], end[k]);
+    }
+  }
+  const int kept = kept_of<LN>(lane), kept_j = kept % ST;
+  const int kept_at = (warp * TT + kept / ST) * 2 * S + Sh::first(q, kept_j / 4) + kept_j % 4;      // in part[][][][]
+  const bool keeps = LN > 2 || lane < 16;      // (sixteen groups: two lanes have the same sum)
+  // the states in front of the eight steps that are next
+  u64 ck[C][NP];
+  auto checkpoint = [&](int t) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) ck[c][i] = 0ull;
+      if (c < mine && t >= t_first && t < t_end)
+        load_states<Sh>(p.ckpt + (((long long)at.n * nck + t / KT) * p.D + d + c) * S, q, ck[c]);
+    }
+  };
+  checkpoint(t_first + (t_end - t_first - 1) / KT * KT);
+  unsigned resets = reset_bits(p, at.n, t_last, t_end - t_last);
+  __syncthreads();
+
+  for (int t0 = t_last, k0 = 0; t0 >= t_first; t0 -= TT, k0 ^= 1) {
+    auto& tl = sm.tile[k0];
+    const int steps = min(TT, t_end - t0);
+    const unsigned now = resets;
+    if (t0 - TT >= t_first) resets = reset_bits(p, at.n, t0 - TT, TT);
+    float* part_mine = &tl.part[0][0][0][0] + kept_at;
+
+    // Four steps at a time, the last first.  The second four of eight have the first four walked on the way to them (without what they
+    // leave), so that a and a h of no more than four stay in registers.
+    auto eights = [&](auto whole) __attribute__((always_inline)) {
+      constexpr bool WHOLE = decltype(whole)::value;
+#pragma unroll 1
+      for (int s0 = TT - SUB; s0 >= 0; s0 -= SUB) {
+        if (!WHOLE && s0 >= steps) continue;
+        u64 h[C][NP];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int i = 0; i < NP; ++i) h[c][i] = ck[c][i];
+        if (s0 % KT != 0) {
+          u64 a[SUB][C][NP], in[SUB][C][NP];      // (first what does not wait for the state)
+#pragma unroll
+          for (int k = 0; k < SUB; ++k) {
+            float2 x[C];
+            load_channels<C>(&tl.dd[s0 - SUB + k][chl], x);
+            u64 b2[NP];
+            load_states<Sh>(&tl.bc[0][s0 - SUB + k][0], q, b2);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const u64 d2 = dup2(x[c].x), x2 = dup2(x[c].y);
+#pragma unroll
+              for (int i = 0; i < NP; ++i) {
+                a[k][c][i] = exp2_pair(mul2(d2, A2[c][i]));
+                in[k][c][i] = mul2(x2, b2[i]);
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < SUB; ++k) {
+            const bool fresh = !WHOLE && (now >> (s0 - SUB + k) & 1u);
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+              for (int i = 0; i < NP; ++i) h[c][i] = fresh ? in[k][c][i] : fma2<true>(a[k][c][i], h[c][i], in[k][c][i]);
+          }
+        } else {
+          checkpoint(t0 + s0 - KT);
+        }
+        u64 a[SUB][C][NP], ah[SUB][C][NP];      // ah: what is inserted first, then a h
+#pragma unroll
+        for (int k = 0; k < SUB; ++k) {
+          float2 x[C];
+          load_channels<C>(&tl.dd[s0 + k][chl], x);
+          u64 b2[NP];
+          load_states<Sh>(&tl.bc[0][s0 + k][0], q, b2);
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const u64 d2 = dup2(x[c].x), x2 = dup2(x[c].y);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+              a[k][c][i] = exp2_pair(mul2(d2, A2[c][i]));
+              ah[k][c][i] = mul2(x2, b2[i]);
+            }
+          }
+        }
+        float dc[8], yv[C][LN];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int i = 0; i < LN; ++i) yv[c][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < SUB; ++k) {
+          const int t = s0 + k;
+          float* dck = dc + k % GS * ST;
+#pragma unroll
+          for (int i = 0; i < ST; ++i) dck[i] = 0.f;
+          if (WHOLE || t < steps) {
+            const bool fresh = !WHOLE && (now >> t & 1u);
+            u64 c2[NP], sum[NP];
+            load_states<Sh>(&tl.bc[1][t][0], q, c2);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const u64 g2 = dup2(tl.gy[t][chl + c]);
+              u64 acc = 0ull;
+#pragma unroll
+              for (int i = 0; i < NP; ++i) {
+                const u64 in = ah[k][c][i];
+                if (fresh) a[k][c][i] = h[c][i] = 0ull;
+                ah[k][c][i] = mul2(a[k][c][i], h[c][i]);
+                h[c][i] = add2(ah[k][c][i], in);
+                acc = i == 0 ? mul2(h[c][i], c2[i]) : fma2<true>(h[c][i], c2[i], acc);
+                sum[i] = c == 0 ? mul2(h[c][i], g2) : fma2<true>(h[c][i], g2, sum[i]);
+              }
+              yv[c][k % LN] = hsum2(acc);
+            }
+#pragma unroll
+            for (int i = 0; i < NP; ++i) unpack2(sum[i], dck[2 * i], dck[2 * i + 1]);
+          }
+          if (k % GS == GS - 1) {
+            groups_to_lanes<LN>(dc, lane);
+            float* o = part_mine + (s0 + k - (GS - 1)) * 2 * S + S;
+            if (keeps) {
+#pragma unroll
+              for (int i = 0; i < KEPT; ++i) o[i] = dc[i];
+            }
+          }
+          if (gate && (k % LN == LN - 1 || k == SUB - 1)) {      // (eight lanes: the values of the four that there are no steps for are zero)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const float y = steps_to_lanes<LN>(yv[c], q);
+              if (q < SUB) tl.yp[s0 + k - (LN < SUB ? LN : SUB) + 1 + q][chl + c] = y;
+            }
+          }
+        }
+        float db[8], gbv[C][LN], sav[C][LN];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int i = 0; i < LN; ++i) gbv[c][i] = sav[c][i] = 0.f;
+#pragma unroll
+        for (int k = SUB - 1; k >= 0; --k) {
+          const int t = s0 + k;
+          float* dbk = db + k % GS * ST;
+#pragma unroll
+          for (int i = 0; i < ST; ++i) dbk[i] = 0.f;
+#pragma unroll
+          for (int c = 0; c < C; ++c) gbv[c][k % LN] = sav[c][k % LN] = 0.f;
+          if (WHOLE || t < steps) {
+            float2 x[C];
+            load_channels<C>(&tl.dd[t][chl], x);
+            u64 b2[NP], c2[NP], sum[NP];
+            load_states<Sh>(&tl.bc[0][t][0], q, b2);
+            load_states<Sh>(&tl.bc[1][t][0], q, c2);
+            const bool fresh = !WHOLE && (now >> t & 1u);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const u64 d2 = dup2(x[c].x), x2 = dup2(x[c].y), g2 = dup2(tl.gy[t][chl + c]);
+              u64 gb = 0ull, sa = 0ull;
+#pragma unroll
+              for (int i = 0; i < NP; ++i) {
+                const u64 g = fma2<true>(c2[i], g2, gc[c][i]), gah = mul2(g, ah[k][c][i]);
+                gb = i == 0 ? mul2(g, b2[i]) : fma2<true>(g, b2[i], gb);
+                sa = i == 0 ? mul2(gah, A2[c][i]) : fma2<true>(gah, A2[c][i], sa);
+                dA[c][i] = fma2<true>(gah, d2, dA[c][i]);
+                sum[i] = c == 0 ? mul2(g, x2) : fma2<true>(g, x2, sum[i]);
+                gc[c][i] = fresh ? 0ull : mul2(a[k][c][i], g);
+              }
+              gbv[c][k % LN] = hsum2(gb);
+              sav[c][k % LN] = hsum2(sa);
+            }
+#pragma unroll
+            for (int i = 0; i < NP; ++i) unpack2(sum[i], dbk[2 * i], dbk[2 * i + 1]);
+          }
+          if (k % GS == 0) {
+            groups_to_lanes<LN>(db, lane);
+            float* o = part_mine + (s0 + k) * 2 * S;
+            if (keeps) {
+#pragma unroll
+              for (int i = 0; i < KEPT; ++i) o[i] = db[i];
+            }
+          }
+          if (k % LN == 0) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const float g = steps_to_lanes<LN>(gbv[c], q), s = steps_to_lanes<LN>(sav[c], q);
+              if (q < SUB) {
+                tl.gb[s0 + k + q][chl + c] = g;
+                tl.sa[s0 + k + q][chl + c] = s * 0.6931471805599453f;      // (A2 has log2(e) in it)
+              }
+            }
+          }
+        }
+      }
+    };
+    if (steps == TT && now == 0u) eights(std::true_type());
+    else eights(std::false_type());
+    __syncthreads();
+  }
+  const long long slot = (long long)at.n * p.nseg + seg;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (c >= mine) continue;
+    store_states<Sh>(p.part_a + (slot * p.D + d + c) * S, q, dA[c]);
+    if (seg == 0 && p.dh0) store_states<Sh>(p.dh0 + own + c * S, q, gc[c]);
+  }
+}
+
+template <typename T, int S, bool VEC>
+__global__ void __launch_bounds__(BwdShape<S>::NT, BwdRegs<T, S>::CTAS) scan_bwd_kernel(const ScanParams p) {
+  extern __shared__ __align__(16) unsigned char raw_smem[];
+  BwdSmem<S>& sm = *reinterpret_cast<BwdSmem<S>*>(raw_smem);
+  if (threadIdx.x >= BwdShape<S>::WALK) {
+    fewer_registers<BwdRegs<T, S>::LOADERS>();
+    scan_bwd_load<T, S, VEC>(p, sm);
+  } else {
+    more_registers<BwdRegs<T, S>::WALKERS>();
+    scan_bwd_walk<T, S, VEC>(p, sm);
   }
 }
 
 // What a piece of the time axis adds to the gradient of the state in front of it (from zero behind it), and the product of its
 // decays, for pieces 1 .. nseg - 1.
 template <typename T, int S, bool VEC>
-__global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_carry_kernel(const ScanParams p) {
-  using Sh = Shape<S>;
-  constexpr int TT = SCAN_TILE, CH = SCAN_CH, NP = Sh::ST / 2, NQ = (Sh::QUADS / 2 + Sh::NT - 1) / Sh::NT;
-  __shared__ __align__(16) float4 dg[2][TT][CH];        // Delta twice, dy' twice
+__global__ void __launch_bounds__(BwdShape<S>::NT) scan_bwd_carry_kernel(const ScanParams p) {
+  using Sh = BwdShape<S>;
+  constexpr int TT = SCAN_TILE, CH = Sh::CH, C = Sh::C, NP = Sh::NP, NL = Sh::NL, NQ = Sh::NQ;
+  __shared__ __align__(16) float2 dg[2][TT][CH];        // Delta, dy'
   __shared__ __align__(16) float cs[2][TT][S];
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, q = lane % Sh::LN, chl = warp * Sh::LC + lane / Sh::LN;
-  const Place at(p, blockIdx.x);
+  const Place<CH> at(p, blockIdx.x);
   const int seg = blockIdx.y + 1, t_first = seg * p.seglen, t_end = min(p.L, t_first + p.seglen);
   const int t_last = t_first + (t_end - t_first - 1) / TT * TT;
-  const bool mine = chl < at.left;
-  const int d = at.ch0 + chl, here = swizzled(chl);
-  const bool loader = tid < TT * CH / 4;
-  const int row = tid / (CH / 4), col = tid % (CH / 4) * 4, valid = loader ? max(0, min(4, at.left - col)) : 0;
-  auto rows = [&](const ScanRows& w) { return reinterpret_cast<const T*>(w.p) + at.n * w.sn + (t_last + row) * w.sl + at.ch0 + col; };
-  const T *pd = rows(p.delta), *pz = rows(p.z), *py = rows(p.dy);
+  if (threadIdx.x >= Sh::WALK) {
+  const int tid = threadIdx.x - Sh::WALK;
   const bool gate = p.z.p != nullptr;
-  float bias[4];
+  int row[NL], col[NL], valid[NL];
+  float bias[NL][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bias[i] = i < valid && p.bias ? p.bias[at.ch0 + col + i] : 0.f;
-  const T* pc[NQ];
+  for (int k = 0; k < NL; ++k) {
+    const int id = tid + k * Sh::LOAD;
+    row[k] = id / (CH / 4);
+    col[k] = id % (CH / 4) * 4;
+    valid[k] = max(0, min(4, at.left - col[k]));
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    const int id = tid + i * Sh::NT;
-    pc[i] = reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + (t_last + id / (S / 4)) * p.C.sl + id % (S / 4) * 4;
+    for (int i = 0; i < 4; ++i) bias[k][i] = p.bias && i < valid[k] ? p.bias[at.ch0 + col[k] + i] : 0.f;
   }
-  Quad<T, VEC> fd, fz, fy, fc[NQ];
+  auto place = [&](const ScanRows& w, int t, int k) { return reinterpret_cast<const T*>(w.p) + at.n * w.sn + t * w.sl + at.ch0 + col[k]; };
+  Quad<T, VEC> fd[NL], fz[NL], fy[NL], fc[NQ];
   auto fetch = [&](int t0) {
-    const int v = t0 + row < t_end ? valid : 0;
-    fd.fetch(pd, v);
-    fy.fetch(py, v);
-    if (gate) fz.fetch(pz, v);
-    pd -= TT * p.delta.sl; py -= TT * p.dy.sl; pz -= TT * p.z.sl;
+#pragma unroll
+    for (int k = 0; k < NL; ++k) {
+      const int t = t0 + row[k], v = t < t_end ? valid[k] : 0;
+      fd[k].fetch(place(p.delta, t, k), v);
+      fy[k].fetch(place(p.dy, t, k), v);
+      if (gate) fz[k].fetch(place(p.z, t, k), v);
+    }
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      const int r = (tid + i * Sh::NT) / (S / 4);
-      fc[i].fetch(pc[i], r < TT && t0 + r < t_end ? 4 : 0);
-      pc[i] -= TT * p.C.sl;
+      const int id = tid + i * Sh::LOAD, t = t0 + id / (S / 4);
+      fc[i].fetch(reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + t * p.C.sl + id % (S / 4) * 4, id < Sh::QUADS && t < t_end ? 4 : 0);
     }
   };
   auto stage = [&](int buf) {
-    if (loader) {
-      const float4 r4 = fd.get(), y4 = fy.get();
-      u64 lo = add2(pack2(r4.x, r4.y), pack2(bias[0], bias[1])), hi = add2(pack2(r4.z, r4.w), pack2(bias[2], bias[3]));
+#pragma unroll
+    for (int k = 0; k < NL; ++k) {
+      const float4 r4 = fd[k].get();
+      float4 g = fy[k].get();
+      u64 lo = add2(pack2(r4.x, r4.y), pack2(bias[k][0], bias[k][1])), hi = add2(pack2(r4.z, r4.w), pack2(bias[k][2], bias[k][3]));
       if (p.softplus) {
         lo = softplus2(lo);
         hi = softplus2(hi);
       }
-      float dl[4], g[4] = {y4.x, y4.y, y4.z, y4.w};
+      float dl[4];
       unpack2(lo, dl[0], dl[1]); unpack2(hi, dl[2], dl[3]);
       if (gate) {
-        const float4 z4 = fz.get();
-        g[0] *= z4.x * sigmoid(z4.x); g[1] *= z4.y * sigmoid(z4.y); g[2] *= z4.z * sigmoid(z4.z); g[3] *= z4.w * sigmoid(z4.w);
+        const float4 z4 = fz[k].get();
+        g.x *= z4.x * sigmoid(z4.x); g.y *= z4.y * sigmoid(z4.y); g.z *= z4.z * sigmoid(z4.z); g.w *= z4.w * sigmoid(z4.w);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) dg[buf][row][swizzled(col + i)] = make_float4(dl[i], dl[i], g[i], g[i]);
+      float4* o = reinterpret_cast<float4*>(&dg[buf][row[k]][col[k]]);
+      o[0] = make_float4(dl[0], g.x, dl[1], g.y);
+      o[1] = make_float4(dl[2], g.z, dl[3], g.w);
     }
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      const int id = tid + i * Sh::NT;
-      if (id < Sh::QUADS / 2) *reinterpret_cast<float4*>(&cs[buf][0][0] + id * 4) = fc[i].get();
+      const int id = tid + i * Sh::LOAD;
+      if (id < Sh::QUADS) *reinterpret_cast<float4*>(&cs[buf][0][0] + id * 4) = fc[i].get();
     }
   };
-  u64 A2[NP], gc[NP];
-#pragma unroll
-  for (int i = 0; i < NP; ++i) A2[i] = gc[i] = 0ull;
-  if (t_first < t_end) fetch(t_last);
-  if (mine) {
-    load_states<Sh>(p.A + (long long)d * S, q, A2);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) A2[i] = mul2(A2[i], dup2(LOG2E));
-  }
-  float sum_d = 0.f;
-  bool cut = false;
-  unsigned resets = 0u;
-  if (t_first < t_end) {
-    stage(0);
-    resets = reset_bits(p, at.n, t_last, t_end - t_last);
-    if (t_last - TT >= t_first) fetch(t_last - TT);
+  fetch(t_last);
+  stage(0);
+  if (t_last - TT >= t_first) fetch(t_last - TT);
+  __syncthreads();
+  for (int t0 = t_last, k0 = 0; t0 >= t_first; t0 -= TT, k0 ^= 1) {
+    if (t0 - TT >= t_first) {
+      stage(k0 ^ 1);
+      if (t0 - 2 * TT >= t_first) fetch(t0 - 2 * TT);
+    }
     __syncthreads();
   }
+  return;
+  }
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, q = lane % Sh::LN, chl = (warp * Sh::LC + lane / Sh::LN) * C;
+  const int d = at.ch0 + chl, mine = at.left - chl;
+  u64 A2[C][NP], gc[C][NP];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) A2[c][i] = gc[c][i] = 0ull;
+    if (c < mine) load_states<Sh>(p.A + (long long)(d + c) * S, q, A2[c]);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) A2[c][i] = mul2(A2[c][i], dup2(LOG2E));
+  }
+  float sum_d[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) sum_d[c] = 0.f;
+  bool cut = false;
+  unsigned resets = reset_bits(p, at.n, t_last, t_end - t_last);
+  __syncthreads();
   for (int t0 = t_last, k0 = 0; t0 >= t_first; t0 -= TT, k0 ^= 1) {
     const int steps = min(TT, t_end - t0);
     const unsigned now = resets;
-    if (t0 - TT >= t_first) {
-      stage(k0 ^ 1);
-      resets = reset_bits(p, at.n, t0 - TT, TT);
-      if (t0 - 2 * TT >= t_first) fetch(t0 - 2 * TT);
-    }
+    if (t0 - TT >= t_first) resets = reset_bits(p, at.n, t0 - TT, TT);
     auto walk = [&](auto whole) {
       constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
       for (int t = TT - 1; t >= 0; --t) {
         if (!WHOLE && t >= steps) continue;
-        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&dg[k0][t][here]);
+        float2 x[C];
+        load_channels<C>(&dg[k0][t][chl], x);
         u64 c2[NP];
         load_states<Sh>(&cs[k0][t][0], q, c2);
         const bool fresh = !WHOLE && (now >> t & 1u);
         cut |= fresh;
-        sum_d += __uint_as_float((unsigned)x.x);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const u64 g = fma2<true>(c2[i], x.y, gc[i]), a = exp2_pair(mul2(x.x, A2[i]));
-          gc[i] = fresh ? 0ull : mul2(a, g);
+        for (int c = 0; c < C; ++c) {
+          const u64 d2 = dup2(x[c].x), g2 = dup2(x[c].y);
+          sum_d[c] += x[c].x;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            const u64 g = fma2<true>(c2[i], g2, gc[c][i]), a = exp2_pair(mul2(d2, A2[c][i]));
+            gc[c][i] = fresh ? 0ull : mul2(a, g);
+          }
         }
       }
     };
@@ -480,19 +616,22 @@ __global__ void __launch_bounds__(Shape<S>::NT) scan_bwd_carry_kernel(const Scan
     else walk(std::false_type());
     __syncthreads();
   }
-  if (!mine) return;
   const long long states = (long long)p.N * p.D * S, own = ((long long)at.n * p.D + d) * S;
-  u64 decay[NP];
 #pragma unroll
-  for (int i = 0; i < NP; ++i) decay[i] = cut ? 0ull : exp2_pair(mul2(dup2(sum_d), A2[i]));
-  store_states<Sh>(p.carry + (2 * seg - 2) * states + own, q, gc);
-  store_states<Sh>(p.carry + (2 * seg - 1) * states + own, q, decay);
+  for (int c = 0; c < C; ++c) {
+    if (c >= mine) continue;
+    u64 decay[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) decay[i] = cut ? 0ull : exp2_pair(mul2(dup2(sum_d[c]), A2[c][i]));
+    store_states<Sh>(p.carry + (2 * seg - 2) * states + own + c * S, q, gc[c]);
+    store_states<Sh>(p.carry + (2 * seg - 1) * states + own + c * S, q, decay);
+  }
 }
 
 // The CTAs' shares added up: blocks below `bc_blocks` four values of dB or dC a thread, the others one of dA, dD or dbias
 template <typename T>
 __global__ void __launch_bounds__(256) scan_sums_kernel(const ScanParams p, int bc_blocks) {
-  const int per = (p.D / p.G + SCAN_CH - 1) / SCAN_CH, GS = p.G * p.S;
+  const int ch = scan_bwd_channels(p.S), per = (p.D / p.G + ch - 1) / ch, GS = p.G * p.S;
   if ((int)blockIdx.x < bc_blocks) {
     const long long rows = (long long)p.N * p.L, total = 2 * rows * GS;
     const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
@@ -527,7 +666,7 @@ __global__ void __launch_bounds__(256) scan_sums_kernel(const ScanParams p, int 
 
 template <typename T, int S, bool VEC>
 cudaError_t launch(const ScanParams& p, cudaStream_t s) {
-  const unsigned grid = (unsigned)(blocks_of(p) * p.N);
+  const unsigned grid = (unsigned)blocks_of(p, BwdShape<S>::CH);
   constexpr int smem = sizeof(BwdSmem<S>);
   static unsigned long long raised = 0;      // devices whose limit is raised
   if (smem > 48 * 1024) {
@@ -541,10 +680,10 @@ cudaError_t launch(const ScanParams& p, cudaStream_t s) {
     }
   }
   if (p.nseg > 1) {
-    scan_bwd_carry_kernel<T, S, VEC><<<dim3(grid, p.nseg - 1), Shape<S>::NT, 0, s>>>(p);
+    scan_bwd_carry_kernel<T, S, VEC><<<dim3(grid, p.nseg - 1), BwdShape<S>::NT, 0, s>>>(p);
     if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   }
-  scan_bwd_kernel<T, S, VEC><<<dim3(grid, p.nseg), Shape<S>::NT, smem, s>>>(p);
+  scan_bwd_kernel<T, S, VEC><<<dim3(grid, p.nseg), BwdShape<S>::NT, smem, s>>>(p);
   if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   const long long quads = 2ll * p.N * p.L * p.G * S / 4, bc_blocks = (quads + 255) / 256;
   const long long rest = ((long long)p.D * S + 2 * p.D + 255) / 256;
@@ -556,7 +695,7 @@ cudaError_t launch(const ScanParams& p, cudaStream_t s) {
 int scan_bwd_segments(int N, int L, int D, int sms) { return scan_segments(N, L, D, sms); }
 
 long long scan_bwd_scratch(ScanParams& p, float* base) {
-  const long long per = (p.D / p.G + SCAN_CH - 1) / SCAN_CH, slots = (long long)p.N * p.nseg;
+  const long long ch = scan_bwd_channels(p.S), per = (p.D / p.G + ch - 1) / ch, slots = (long long)p.N * p.nseg;
   const long long bc = per * 2 * p.N * p.L * p.G * p.S, a = slots * p.D * p.S, v = (slots * 2 * p.D + 3) / 4 * 4;
   const long long carry = p.nseg > 1 ? 2ll * (p.nseg - 1) * p.N * p.D * p.S : 0;
   if (base) {
