@@ -496,7 +496,7 @@ typedef struct srwm_b200_scan_grads {
 int     srwm_b200_scan_forward(const srwm_b200_scan_args* args, void* cuda_stream);
 int     srwm_b200_scan_backward(const srwm_b200_scan_args* args, const srwm_b200_scan_grads* grads, void* cuda_stream);
 int64_t srwm_b200_scan_checkpoint_floats(int32_t N, int32_t L, int32_t D, int32_t S);
-int64_t srwm_b200_scan_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S);
+int64_t srwm_b200_scan_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S, int32_t G);
 int64_t srwm_b200_scan_backward_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S, int32_t G);
 
 /* y_t = act(bias + sum_i w[K-1-i] x_{t-i}), act = silu or the identity, K = 2, 3 or 4 taps (otherwise ERR_SHAPE); w [D, K], bias [D] dense

@@ -964,7 +964,7 @@ static int scan_params(const srwm_b200_scan_args* a, srwm::ScanParams* p, bool b
   p->A = a->A; p->skip = a->skip; p->bias = a->delta_bias; p->h0 = a->state_in; p->hT = a->state_out;
   p->done = a->done; p->done_n = a->done_stride_n; p->done_l = a->done_stride_l;
   p->ckpt = a->checkpoints;
-  p->nseg = backward ? srwm::scan_bwd_segments(a->N, a->L, a->D, srwm::common_sms()) : srwm::scan_segments(a->N, a->L, a->D, srwm::common_sms());
+  p->nseg = srwm::scan_segments(*p, backward ? srwm::scan_bwd_channels(a->S) : srwm::SCAN_FWD_CHANNELS, srwm::common_sms());
   const int per = (a->L + p->nseg - 1) / p->nseg;
   p->seglen = (per + srwm::SCAN_TILE - 1) / srwm::SCAN_TILE * srwm::SCAN_TILE;
   if (p->seglen > 0) p->nseg = (a->L + p->seglen - 1) / p->seglen;      // (rounded up, fewer pieces may do)
@@ -986,8 +986,8 @@ static srwm::ScanParams scan_shape(int32_t N, int32_t L, int32_t D, int32_t S, i
 extern "C" int64_t srwm_b200_scan_checkpoint_floats(int32_t N, int32_t L, int32_t D, int32_t S) {
   return N <= 0 || L <= 0 || D <= 0 || S <= 0 ? 0 : (int64_t)N * ((L + srwm::SCAN_CKPT - 1) / srwm::SCAN_CKPT) * D * S;
 }
-extern "C" int64_t srwm_b200_scan_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S) {
-  return 4 * srwm::scan_fwd_scratch(scan_shape(N, L, D, S, 1, false));
+extern "C" int64_t srwm_b200_scan_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S, int32_t G) {
+  return 4 * srwm::scan_fwd_scratch(scan_shape(N, L, D, S, G, false));
 }
 extern "C" int64_t srwm_b200_scan_backward_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S, int32_t G) {
   srwm::ScanParams p = scan_shape(N, L, D, S, G, true);

@@ -104,7 +104,7 @@ inline variable_list scan_forward(const ScanIn& s, bool inplace, Tensor* checkpo
     *checkpoints = floats(s.u, {api().srwm_b200_scan_checkpoint_floats(a.N, a.L, a.D, a.S)});
     a.checkpoints = floats_in(*checkpoints);
   }
-  if (const int64_t need = api().srwm_b200_scan_scratch_bytes(a.N, a.L, a.D, a.S)) {
+  if (const int64_t need = api().srwm_b200_scan_scratch_bytes(a.N, a.L, a.D, a.S, a.G)) {
     scratch = floats(s.u, {need / 4});
     a.scratch = scratch.data_ptr();
     a.scratch_bytes = need;

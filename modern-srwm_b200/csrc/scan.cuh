@@ -18,9 +18,9 @@ namespace scan {
 
 // C: neighbouring channels of a thread.  A step's B and C are then read once for C channels: with one, the shared-memory pipe (a 16-byte load
 // is four of its cycles) is busier than the exponentials' one.
-template <int S_, int C_>
+template <int S_, int C_, int TT_>
 struct Shape {
-  static constexpr int S = S_, C = C_;
+  static constexpr int S = S_, C = C_, TT = TT_;              // TT: steps of a tile
   static constexpr int LN = S == 8 ? 2 : S == 64 ? 8 : 4;    // lanes of a channel
   static constexpr int ST = S / LN;                           // states of a thread and channel (4 or 8)
   static constexpr int NP = ST / 2;                           // pairs of them
@@ -28,8 +28,11 @@ struct Shape {
   static constexpr int WARPS = LN < 4 ? 4 : LN, WALK = 32 * WARPS;      // warps and threads that walk the time axis
   static constexpr int LOAD = 128, NT = WALK + LOAD;          // threads that load, prepare and write tiles beside them; all
   static constexpr int CH = WARPS * LC * C;                   // channels of a CTA
-  static constexpr int PIECES = SCAN_TILE * CH / 4, NL = PIECES / LOAD;               // pieces of four channels of a tile; of a loading thread
-  static constexpr int QUADS = SCAN_TILE * S / 4, NQ = (QUADS + LOAD - 1) / LOAD;     // pieces of four of B (and of C)
+  static constexpr int PIECES = TT * CH / 4, NL = (PIECES + LOAD - 1) / LOAD;               // pieces of four channels of a tile; of a loading thread
+  static constexpr int QUADS = TT * S / 4, NQ = (QUADS + LOAD - 1) / LOAD;     // pieces of four of B (and of C)
+  // What a channel's lanes add up to goes through shared memory, a row a lane (one store a step; shuffles and selects are five times
+  // the instructions), at a distance that keeps the rows' banks apart
+  static constexpr int PAD = CH + (LN == 2 ? 16 : LN == 4 ? 8 : 4);
   // state j of lane q: whole pieces of four lie side by side over the lanes, so that a warp reads B and C without conflicts
   static __device__ __forceinline__ int first(int q, int piece) { return piece * 4 * LN + q * 4; }
 };
@@ -147,19 +150,21 @@ __device__ __forceinline__ void put4(__nv_bfloat16* p, int valid, float4 v) {
   }
 }
 
-// Sums over a channel's LN lanes of LN steps' values: lane q gets step q's
-template <int LN>
-__device__ __forceinline__ float steps_to_lanes(float* v, int q) {
+// The same step's values of the LN lanes' rows, added up
+template <typename Sh>
+__device__ __forceinline__ float4 sum_lanes(const float* p) {
+  float4 v = *reinterpret_cast<const float4*>(p);
 #pragma unroll
-  for (int w = 1; w < LN; w *= 2) {
-    const bool up = q & w;
-#pragma unroll
-    for (int i = 0; i < LN; i += 2 * w) {
-      const float keep = up ? v[i + w] : v[i], send = up ? v[i] : v[i + w];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
-    }
+  for (int q = 1; q < Sh::LN; ++q) {
+    const float4 o = *reinterpret_cast<const float4*>(p + q * Sh::PAD);
+    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
   }
-  return v[0];
+  return v;
+}
+template <int C>
+__device__ __forceinline__ void store_channels(float* p, const float* v) {
+  if constexpr (C == 2) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+  else *p = v[0];
 }
 
 // A thread's states of a channel as pairs, from or to that channel's [S] floats
@@ -223,6 +228,19 @@ __device__ __forceinline__ unsigned reset_bits(const ScanParams& p, int n, int t
 inline long long blocks_of(const ScanParams& p, int channels) {
   const int Dg = p.D / p.G;
   return (long long)((Dg + channels - 1) / channels) * p.G * p.N;
+}
+
+// Raises a kernel's limit of dynamic shared memory, once a device
+template <typename Kernel>
+inline cudaError_t allow_smem(Kernel kern, int bytes, unsigned long long* raised) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (__atomic_load_n(raised, __ATOMIC_ACQUIRE) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) __atomic_fetch_or(raised, bit, __ATOMIC_RELEASE);
+  return e;
 }
 
 // f(element, states, vec) as types

@@ -34,8 +34,8 @@ struct ScanParams {
 };
 
 __host__ __device__ constexpr int scan_bwd_channels(int S) { return S == 8 ? 128 : S == 16 ? 64 : 32; }      // of a CTA of the backward
-int scan_segments(int N, int L, int D, int sms);          // pieces that a call's time axis is cut into
-int scan_bwd_segments(int N, int L, int D, int sms);
+constexpr int SCAN_FWD_CHANNELS = 64;                     // of a CTA of the forward (32 where these would not fill the GPU)
+int scan_segments(const ScanParams& p, int channels, int sms);      // pieces that a call's time axis is cut into
 long long scan_fwd_scratch(const ScanParams& p);           // floats
 long long scan_bwd_scratch(ScanParams& p, float* base);    // floats; base not NULL: sets the pointers into it
 cudaError_t scan_forward(const ScanParams& p, cudaStream_t s);

@@ -16,52 +16,102 @@ namespace srwm {
 namespace {
 using namespace scan;
 
-// Sums of eight values over a warp's 32 / LN channel groups: 8 values (or one, where there are eight groups or more) stay with each
-// lane, those from index kept_of on
-template <int LN>
-__device__ __forceinline__ void groups_to_lanes(float* v, int lane) {
+// The states of a thread are held in an order of its own: state j of piece i in register (i ^ pp, j ^ (2 x1 + x0)), where pp, x1, x0 are bits of its
+// channel group.  The sums over the warp's groups then halve at each exchange without a select: a lane keeps its first
+// half and sends the second, which is what the other lane keeps.
+template <int ST, int LN>
+struct Order {
+  int pp, x1, x0;
+  __device__ __forceinline__ explicit Order(int lane) {
+    const int c = lane / LN;
+    pp = ST == 8 ? c & 1 : 0;
+    x1 = ST == 8 ? c >> 1 & 1 : c & 1;
+    x0 = ST == 8 ? (LN == 8 ? 0 : c >> 2 & 1) : c >> 1 & 1;
+  }
+  __device__ __forceinline__ int copy() const { return x1 + 2 * x0; }      // of four in shared memory (side by side: no conflicts)
+  __device__ __forceinline__ int state() const { return 2 * x1 + x0; }      // in register 0
+  // into the order and out of it, a piece as two pairs
+  __device__ __forceinline__ void turn(u64& lo, u64& hi) const {
+    float a, b, c, d;
+    unpack2(lo, a, b);
+    unpack2(hi, c, d);
+    const float a1 = x1 ? c : a, b1 = x1 ? d : b, c1 = x1 ? a : c, d1 = x1 ? b : d;
+    lo = pack2(x0 ? b1 : a1, x0 ? a1 : b1);
+    hi = pack2(x0 ? d1 : c1, x0 ? c1 : d1);
+  }
+};
+template <typename Sh, typename O>
+__device__ __forceinline__ void load_turned(const float* p, int q, const O& o, u64* v) {
 #pragma unroll
-  for (int w = LN, half = 4; w < 32; w *= 2, half /= 2) {
-    const bool up = lane & w;
-    if (half == 0) v[0] += __shfl_xor_sync(0xffffffffu, v[0], w);
-#pragma unroll
-    for (int i = 0; i < half; ++i) {
-      const float keep = up ? v[half + i] : v[i], send = up ? v[i] : v[half + i];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
-    }
+  for (int i = 0; i < Sh::ST / 4; ++i) {
+    const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(p + Sh::first(q, i ^ o.pp));
+    v[2 * i] = t.x; v[2 * i + 1] = t.y;
+    o.turn(v[2 * i], v[2 * i + 1]);
   }
 }
-template <int LN>
-__device__ __forceinline__ int kept_of(int lane) {
-  const int c = lane / LN;       // the lowest bit of the group halves first
-  return LN == 8 ? (c & 1) * 4 + (c & 2) : (c & 1) * 4 + (c & 2) + (c >> 2 & 1);
+template <typename Sh, typename O>
+__device__ __forceinline__ void store_turned(float* p, int q, const O& o, const u64* v) {
+#pragma unroll
+  for (int i = 0; i < Sh::ST / 4; ++i) {
+    u64 lo = v[2 * i], hi = v[2 * i + 1];
+    o.turn(lo, hi);
+    *reinterpret_cast<ulonglong2*>(p + Sh::first(q, i ^ o.pp)) = make_ulonglong2(lo, hi);
+  }
+}
+// Sums of eight values (8 / ST steps of a thread's states) over the warp's channel groups: v[0] (and v[1], with four groups) is what
+// the lane keeps
+template <int ST, int LN>
+__device__ __forceinline__ void sum_groups(float* v, int lane) {
+  auto other = [](float x, int w) { return __shfl_xor_sync(0xffffffffu, x, w); };
+  if (ST == 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += other(v[j + 4], LN);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] += other(v[j + 2], 2 * LN);
+    if (LN == 4) v[0] += other(v[1], 4 * LN);
+  } else {
+#pragma unroll
+    for (int s = 0; s < 8; s += 4) {
+      v[s] += other(v[s + 2], LN);
+      v[s + 1] += other(v[s + 3], LN);
+      v[s] += other(v[s + 1], 2 * LN);
+    }
+    const bool up = lane & (4 * LN);       // the second of the two steps
+    const float keep = up ? v[4] : v[0], send = up ? v[0] : v[4];
+    v[0] = keep + other(send, 4 * LN);
+    if (LN == 2) v[0] += other(v[0], 16);
+  }
 }
 
 // Two channels a thread with up to 16 states, one with more: eight states of a thread in all
 template <int S>
-using BwdShape = Shape<S, S <= 16 ? 2 : 1>;
+using BwdShape = Shape<S, S <= 16 ? 2 : 1, SCAN_CKPT>;
+template <int S>
+using BwdCarryShape = Shape<S, S <= 16 ? 2 : 1, SCAN_TILE>;
 
 // Two buffers: a tile is loaded and prepared, and the results of the one before it written, while the tile between is walked
 template <int S>
 struct BwdSmem {
   using Sh = BwdShape<S>;
-  static constexpr int TT = SCAN_TILE, CH = Sh::CH, PAD = CH + 8;
+  static constexpr int TT = Sh::TT, CH = Sh::CH, PAD = Sh::PAD;
   struct Tile {
     float2 dd[TT][CH];           // Delta, Delta u
     float gy[TT][CH];            // dy'
-    float bc[2][TT][S];
-    float gb[TT][PAD], sa[TT][PAD], yp[TT][PAD];
+    float bc[2][TT][4][S];       // B and C, in the four orders of a piece's states
+    float gb[TT][Sh::LN][PAD], sa[TT][Sh::LN][PAD], yp[TT][Sh::LN][PAD];      // g . B, A . (g a h), C . h: a row of each lane of a channel
     float part[Sh::WARPS][TT][2][S];
   } tile[2];
   float4 sums[2][Sh::PIECES];    // of dy' u and of the gradient of delta, a slot for each loading thread's piece
 };
 
-// Registers: the walking threads' share and the loading threads', which together are what the CTA is launched with (128 a thread, two CTAs
-// a multiprocessor; S 64: 168 and one)
-template <typename T, int S>
+// Registers: the walking threads' share and the loading threads', which together are at most what the CTA is launched with (128 a thread, two
+// CTAs a multiprocessor; S 64: 168 and one): a share beyond that would be waited for without end.
+template <int S>
 struct BwdRegs {
-  static constexpr int CTAS = S == 64 ? 1 : 2, LOADERS = 104;
-  static constexpr int WALKERS = S == 64 ? 200 : 256 - LOADERS;
+  using Sh = BwdShape<S>;
+  static constexpr int CTAS = S == 64 ? 1 : 2, LOADERS = 104, WALKERS = S == 64 ? 200 : 152;
+  static constexpr int ALL = Sh::WALK * WALKERS + Sh::LOAD * LOADERS;
+  static_assert(ALL <= 65536 / CTAS / Sh::NT / 8 * 8 * Sh::NT, "more registers than the CTA is launched with");
 };
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -71,7 +121,7 @@ __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec
 template <typename T, int S, bool VEC>
 __device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& sm) {
   using Sh = BwdShape<S>;
-  constexpr int TT = SCAN_TILE, CH = Sh::CH, NL = Sh::NL, NQ = Sh::NQ;
+  constexpr int TT = Sh::TT, CH = Sh::CH, NL = Sh::NL, NQ = Sh::NQ;
   const int tid = threadIdx.x - Sh::WALK;
   const Place<CH> at(p, blockIdx.x);
   const int seg = blockIdx.y, t_first = seg * p.seglen, t_end = min(p.L, t_first + p.seglen);
@@ -80,9 +130,12 @@ __device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& s
   // piece k: row (tid + k LOAD) / (CH / 4), columns from (tid % (CH / 4)) * 4 on
   static_assert(Sh::LOAD % (CH / 4) == 0, "all pieces of a thread have the same columns");
   constexpr int RS = Sh::LOAD / (CH / 4);       // rows between a thread's pieces
-  const int row = tid / (CH / 4), col = tid % (CH / 4) * 4, valid = max(0, min(4, at.left - col));
+  const bool loads = tid < Sh::PIECES;          // (32 channels: half of the threads have a piece)
+  const int row = tid / (CH / 4), col = tid % (CH / 4) * 4, valid = loads ? max(0, min(4, at.left - col)) : 0;
+  if (loads) {
 #pragma unroll
-  for (int k = 0; k < NL; ++k) sm.sums[0][tid + k * Sh::LOAD] = sm.sums[1][tid + k * Sh::LOAD] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < NL; ++k) sm.sums[0][tid + k * Sh::LOAD] = sm.sums[1][tid + k * Sh::LOAD] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   auto place = [&](const ScanRows& w, int t) { return reinterpret_cast<T*>(w.p) + at.n * w.sn + t * w.sl + at.ch0 + col; };
   float bias[4], skip[4];
 #pragma unroll
@@ -113,6 +166,7 @@ __device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& s
     auto& tl = sm.tile[buf];
 #pragma unroll
     for (int k = 0; k < NL; ++k) {
+      if (!loads) break;
       const float4 u4 = fu[k].get(), r4 = fd[k].get();
       u64 lo = add2(pack2(r4.x, r4.y), pack2(bias[0], bias[1])), hi = add2(pack2(r4.z, r4.w), pack2(bias[2], bias[3]));
       if (p.softplus) {
@@ -135,10 +189,17 @@ __device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& s
     }
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      const int id = tid + i * Sh::LOAD;
+      const int id = tid + i * Sh::LOAD, c = id % (S / 4) * 4, r = id / (S / 4);
       if (id >= Sh::QUADS) continue;
-      *reinterpret_cast<float4*>(&tl.bc[0][0][0] + id * 4) = fb[i].get();
-      *reinterpret_cast<float4*>(&tl.bc[1][0][0] + id * 4) = fc[i].get();
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const float4 v = w ? fc[i].get() : fb[i].get();
+        float* o = &tl.bc[w][r][0][c];
+        *reinterpret_cast<float4*>(o) = v;
+        *reinterpret_cast<float4*>(o + S) = make_float4(v.z, v.w, v.x, v.y);
+        *reinterpret_cast<float4*>(o + 2 * S) = make_float4(v.y, v.x, v.w, v.z);
+        *reinterpret_cast<float4*>(o + 3 * S) = make_float4(v.w, v.z, v.y, v.x);
+      }
     }
   };
   auto finish = [&](int t0, int buf) {
@@ -168,7 +229,7 @@ __device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& s
         q2.fetch(place(p.z, t), v);
         q3.fetch(place(p.dy, t), v);
       }
-      const float4 gb4 = *reinterpret_cast<const float4*>(&tl.gb[r][col]), sa4 = *reinterpret_cast<const float4*>(&tl.sa[r][col]);
+      const float4 gb4 = sum_lanes<Sh>(&tl.gb[r][0][col]), sa4 = sum_lanes<Sh>(&tl.sa[r][0][col]);
       const float4 g4 = *reinterpret_cast<const float4*>(&tl.gy[r][col]);
       const float4* dk = reinterpret_cast<const float4*>(&tl.dd[r][col]);
       const float4 d01 = dk[0], d23 = dk[1], u4 = q0.get(), r4 = q1.get();
@@ -178,7 +239,7 @@ __device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& s
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         o1[i] = fmaf(g[i], skip[i], dl[i] * gb[i]);
-        o2[i] = fmaf(us[i], gb[i], sa[i]);
+        o2[i] = fmaf(us[i], gb[i], sa[i] * 0.6931471805599453f);      // (the walking threads' A has log2(e) in it)
         if (p.softplus) o2[i] *= sigmoid(rs[i] + bias[i]);
       }
       put4<VEC>(place(p.du, t), v, make_float4(o1[0], o1[1], o1[2], o1[3]));
@@ -189,7 +250,7 @@ __device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& s
       w = sm.sums[1][id];
       sm.sums[1][id] = make_float4(w.x + o2[0], w.y + o2[1], w.z + o2[2], w.w + o2[3]);
       if (gate) {
-        const float4 yp4 = *reinterpret_cast<const float4*>(&tl.yp[r][col]), z4 = q2.get(), y4 = q3.get();
+        const float4 yp4 = sum_lanes<Sh>(&tl.yp[r][0][col]), z4 = q2.get(), y4 = q3.get();
         const float yp[4] = {yp4.x, yp4.y, yp4.z, yp4.w}, zs[4] = {z4.x, z4.y, z4.z, z4.w}, os[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -236,14 +297,16 @@ __device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& s
 template <typename T, int S, bool VEC>
 __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& sm) {
   using Sh = BwdShape<S>;
-  constexpr int TT = SCAN_TILE, CH = Sh::CH, KT = SCAN_CKPT, C = Sh::C, NP = Sh::NP, ST = Sh::ST, LN = Sh::LN;
-  constexpr int SUB = 4, GS = 8 / ST, KEPT = LN == 8 ? 2 : 1;
+  constexpr int TT = Sh::TT, CH = Sh::CH, C = Sh::C, NP = Sh::NP, ST = Sh::ST, LN = Sh::LN;
+  constexpr int SUB = 4, GS = 8 / ST;
+  static_assert(TT == SCAN_CKPT && TT == 2 * SUB, "a tile's steps are those between two of the forward's states");
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, q = lane % LN, chl = (warp * Sh::LC + lane / LN) * C;
   const Place<CH> at(p, blockIdx.x);
   const int seg = blockIdx.y, t_first = seg * p.seglen, t_end = min(p.L, t_first + p.seglen);
   const int t_last = t_first + (t_end - t_first - 1) / TT * TT;
   const int d = at.ch0 + chl, mine = at.left - chl;
   const bool gate = p.z.p != nullptr;
+  const Order<ST, LN> order(lane);
 
   u64 A2[C][NP], gc[C][NP], dA[C][NP];
 #pragma unroll
@@ -251,39 +314,44 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
 #pragma unroll
     for (int i = 0; i < NP; ++i) A2[c][i] = gc[c][i] = dA[c][i] = 0ull;
   const long long states = (long long)p.N * p.D * S, own = ((long long)at.n * p.D + d) * S;
-  const int nck = (p.L + KT - 1) / KT;
+  const int nck = (p.L + TT - 1) / TT;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     if (c >= mine) continue;
-    load_states<Sh>(p.A + (long long)(d + c) * S, q, A2[c]);
+    load_turned<Sh>(p.A + (long long)(d + c) * S, q, order, A2[c]);
 #pragma unroll
     for (int i = 0; i < NP; ++i) A2[c][i] = mul2(A2[c][i], dup2(LOG2E));
     const long long o = own + c * S;
-    if (p.dhT) load_states<Sh>(p.dhT + o, q, gc[c]);
+    if (p.dhT) load_turned<Sh>(p.dhT + o, q, order, gc[c]);
 #pragma unroll 4
     for (int i = p.nseg - 1; i > seg; --i) {      // the pieces behind, the last first
       u64 decay[NP], end[NP];
-      load_states<Sh>(p.carry + (2 * i - 2) * states + o, q, end);
-      load_states<Sh>(p.carry + (2 * i - 1) * states + o, q, decay);
+      load_turned<Sh>(p.carry + (2 * i - 2) * states + o, q, order, end);
+      load_turned<Sh>(p.carry + (2 * i - 1) * states + o, q, order, decay);
 #pragma unroll
       for (int k = 0; k < NP; ++k) gc[c][k] = fma2<true>(decay[k], gc[c][k], end[k]);
     }
   }
-  const int kept = kept_of<LN>(lane), kept_j = kept % ST;
-  const int kept_at = (warp * TT + kept / ST) * 2 * S + Sh::first(q, kept_j / 4) + kept_j % 4;      // in part[][][][]
+  // in part[][][][]: of v[0] of sum_groups (ST 4: of the step that the lane keeps)
+  const int kept_at = (warp * TT + (ST == 4 ? lane / LN >> 2 & 1 : 0)) * 2 * S + Sh::first(q, order.pp) + order.state();
   const bool keeps = LN > 2 || lane < 16;      // (sixteen groups: two lanes have the same sum)
-  // the states in front of the eight steps that are next
-  u64 ck[C][NP];
+  const int bc_at = order.copy() * S;
+  u64 ck[C][NP];      // the states in front of the next tile
   auto checkpoint = [&](int t) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
       for (int i = 0; i < NP; ++i) ck[c][i] = 0ull;
-      if (c < mine && t >= t_first && t < t_end)
-        load_states<Sh>(p.ckpt + (((long long)at.n * nck + t / KT) * p.D + d + c) * S, q, ck[c]);
+      if (c >= mine || t < t_first) continue;
+#pragma unroll
+      for (int i = 0; i < ST / 4; ++i) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p.ckpt + (((long long)at.n * nck + t / TT) * p.D + d + c) * S + Sh::first(q, i ^ order.pp));
+        ck[c][2 * i] = v.x;
+        ck[c][2 * i + 1] = v.y;
+      }
     }
   };
-  checkpoint(t_first + (t_end - t_first - 1) / KT * KT);
+  checkpoint(t_last);
   unsigned resets = reset_bits(p, at.n, t_last, t_end - t_last);
   __syncthreads();
 
@@ -293,27 +361,45 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
     const unsigned now = resets;
     if (t0 - TT >= t_first) resets = reset_bits(p, at.n, t0 - TT, TT);
     float* part_mine = &tl.part[0][0][0][0] + kept_at;
+    u64 start[C][NP];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < NP; i += 2) {
+        start[c][i] = ck[c][i];
+        start[c][i + 1] = ck[c][i + 1];
+        order.turn(start[c][i], start[c][i + 1]);
+      }
+    checkpoint(t0 - TT);
+    auto load_bc = [&](int w, int t, u64* v) {
+#pragma unroll
+      for (int i = 0; i < ST / 4; ++i) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&tl.bc[w][t][0][0] + bc_at + Sh::first(q, i ^ order.pp));
+        v[2 * i] = x.x;
+        v[2 * i + 1] = x.y;
+      }
+    };
 
-    // Four steps at a time, the last first.  The second four of eight have the first four walked on the way to them (without what they
-    // leave), so that a and a h of no more than four stay in registers.
-    auto eights = [&](auto whole) __attribute__((always_inline)) {
+    // Four steps at a time, the last first.  The second four have the first four walked on the way to them (without what they leave), so that a
+    // and a h of no more than four stay in registers.
+    auto tile = [&](auto whole) __attribute__((always_inline)) {
       constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll 1
-      for (int s0 = TT - SUB; s0 >= 0; s0 -= SUB) {
+      for (int s0 = SUB; s0 >= 0; s0 -= SUB) {
         if (!WHOLE && s0 >= steps) continue;
         u64 h[C][NP];
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-          for (int i = 0; i < NP; ++i) h[c][i] = ck[c][i];
-        if (s0 % KT != 0) {
+          for (int i = 0; i < NP; ++i) h[c][i] = start[c][i];
+        if (s0 > 0) {
           u64 a[SUB][C][NP], in[SUB][C][NP];      // (first what does not wait for the state)
 #pragma unroll
           for (int k = 0; k < SUB; ++k) {
             float2 x[C];
-            load_channels<C>(&tl.dd[s0 - SUB + k][chl], x);
+            load_channels<C>(&tl.dd[k][chl], x);
             u64 b2[NP];
-            load_states<Sh>(&tl.bc[0][s0 - SUB + k][0], q, b2);
+            load_bc(0, k, b2);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
               const u64 d2 = dup2(x[c].x), x2 = dup2(x[c].y);
@@ -326,14 +412,12 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
           }
 #pragma unroll
           for (int k = 0; k < SUB; ++k) {
-            const bool fresh = !WHOLE && (now >> (s0 - SUB + k) & 1u);
+            const bool fresh = !WHOLE && (now >> k & 1u);
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
               for (int i = 0; i < NP; ++i) h[c][i] = fresh ? in[k][c][i] : fma2<true>(a[k][c][i], h[c][i], in[k][c][i]);
           }
-        } else {
-          checkpoint(t0 + s0 - KT);
         }
         u64 a[SUB][C][NP], ah[SUB][C][NP];      // ah: what is inserted first, then a h
 #pragma unroll
@@ -341,7 +425,7 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
           float2 x[C];
           load_channels<C>(&tl.dd[s0 + k][chl], x);
           u64 b2[NP];
-          load_states<Sh>(&tl.bc[0][s0 + k][0], q, b2);
+          load_bc(0, s0 + k, b2);
 #pragma unroll
           for (int c = 0; c < C; ++c) {
             const u64 d2 = dup2(x[c].x), x2 = dup2(x[c].y);
@@ -352,21 +436,16 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
             }
           }
         }
-        float dc[8], yv[C][LN];
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int i = 0; i < LN; ++i) yv[c][i] = 0.f;
+        float v8[8];
 #pragma unroll
         for (int k = 0; k < SUB; ++k) {
           const int t = s0 + k;
-          float* dck = dc + k % GS * ST;
-#pragma unroll
-          for (int i = 0; i < ST; ++i) dck[i] = 0.f;
+          float* vk = v8 + k % GS * ST;
           if (WHOLE || t < steps) {
             const bool fresh = !WHOLE && (now >> t & 1u);
             u64 c2[NP], sum[NP];
-            load_states<Sh>(&tl.bc[1][t][0], q, c2);
+            float y[C];
+            load_bc(1, t, c2);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
               const u64 g2 = dup2(tl.gy[t][chl + c]);
@@ -380,46 +459,33 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
                 acc = i == 0 ? mul2(h[c][i], c2[i]) : fma2<true>(h[c][i], c2[i], acc);
                 sum[i] = c == 0 ? mul2(h[c][i], g2) : fma2<true>(h[c][i], g2, sum[i]);
               }
-              yv[c][k % LN] = hsum2(acc);
+              y[c] = hsum2(acc);
             }
+            if (gate) store_channels<C>(&tl.yp[t][q][chl], y);
 #pragma unroll
-            for (int i = 0; i < NP; ++i) unpack2(sum[i], dck[2 * i], dck[2 * i + 1]);
+            for (int i = 0; i < NP; ++i) unpack2(sum[i], vk[2 * i], vk[2 * i + 1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < ST; ++i) vk[i] = 0.f;
           }
           if (k % GS == GS - 1) {
-            groups_to_lanes<LN>(dc, lane);
-            float* o = part_mine + (s0 + k - (GS - 1)) * 2 * S + S;
-            if (keeps) {
-#pragma unroll
-              for (int i = 0; i < KEPT; ++i) o[i] = dc[i];
-            }
-          }
-          if (gate && (k % LN == LN - 1 || k == SUB - 1)) {      // (eight lanes: the values of the four that there are no steps for are zero)
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-              const float y = steps_to_lanes<LN>(yv[c], q);
-              if (q < SUB) tl.yp[s0 + k - (LN < SUB ? LN : SUB) + 1 + q][chl + c] = y;
-            }
+            sum_groups<ST, LN>(v8, lane);
+            float* o = part_mine + (t - (GS - 1)) * 2 * S + S;
+            if (LN == 8) *reinterpret_cast<float2*>(o) = make_float2(v8[0], v8[1]);
+            else if (keeps) *o = v8[0];
           }
         }
-        float db[8], gbv[C][LN], sav[C][LN];
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int i = 0; i < LN; ++i) gbv[c][i] = sav[c][i] = 0.f;
 #pragma unroll
         for (int k = SUB - 1; k >= 0; --k) {
           const int t = s0 + k;
-          float* dbk = db + k % GS * ST;
-#pragma unroll
-          for (int i = 0; i < ST; ++i) dbk[i] = 0.f;
-#pragma unroll
-          for (int c = 0; c < C; ++c) gbv[c][k % LN] = sav[c][k % LN] = 0.f;
+          float* vk = v8 + k % GS * ST;
           if (WHOLE || t < steps) {
             float2 x[C];
             load_channels<C>(&tl.dd[t][chl], x);
             u64 b2[NP], c2[NP], sum[NP];
-            load_states<Sh>(&tl.bc[0][t][0], q, b2);
-            load_states<Sh>(&tl.bc[1][t][0], q, c2);
+            float gbv[C], sav[C];
+            load_bc(0, t, b2);
+            load_bc(1, t, c2);
             const bool fresh = !WHOLE && (now >> t & 1u);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
@@ -434,55 +500,48 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
                 sum[i] = c == 0 ? mul2(g, x2) : fma2<true>(g, x2, sum[i]);
                 gc[c][i] = fresh ? 0ull : mul2(a[k][c][i], g);
               }
-              gbv[c][k % LN] = hsum2(gb);
-              sav[c][k % LN] = hsum2(sa);
+              gbv[c] = hsum2(gb);
+              sav[c] = hsum2(sa);
             }
+            store_channels<C>(&tl.gb[t][q][chl], gbv);
+            store_channels<C>(&tl.sa[t][q][chl], sav);
 #pragma unroll
-            for (int i = 0; i < NP; ++i) unpack2(sum[i], dbk[2 * i], dbk[2 * i + 1]);
+            for (int i = 0; i < NP; ++i) unpack2(sum[i], vk[2 * i], vk[2 * i + 1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < ST; ++i) vk[i] = 0.f;
           }
           if (k % GS == 0) {
-            groups_to_lanes<LN>(db, lane);
-            float* o = part_mine + (s0 + k) * 2 * S;
-            if (keeps) {
-#pragma unroll
-              for (int i = 0; i < KEPT; ++i) o[i] = db[i];
-            }
-          }
-          if (k % LN == 0) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-              const float g = steps_to_lanes<LN>(gbv[c], q), s = steps_to_lanes<LN>(sav[c], q);
-              if (q < SUB) {
-                tl.gb[s0 + k + q][chl + c] = g;
-                tl.sa[s0 + k + q][chl + c] = s * 0.6931471805599453f;      // (A2 has log2(e) in it)
-              }
-            }
+            sum_groups<ST, LN>(v8, lane);
+            float* o = part_mine + t * 2 * S;
+            if (LN == 8) *reinterpret_cast<float2*>(o) = make_float2(v8[0], v8[1]);
+            else if (keeps) *o = v8[0];
           }
         }
       }
     };
-    if (steps == TT && now == 0u) eights(std::true_type());
-    else eights(std::false_type());
+    if (steps == TT && now == 0u) tile(std::true_type());
+    else tile(std::false_type());
     __syncthreads();
   }
   const long long slot = (long long)at.n * p.nseg + seg;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     if (c >= mine) continue;
-    store_states<Sh>(p.part_a + (slot * p.D + d + c) * S, q, dA[c]);
-    if (seg == 0 && p.dh0) store_states<Sh>(p.dh0 + own + c * S, q, gc[c]);
+    store_turned<Sh>(p.part_a + (slot * p.D + d + c) * S, q, order, dA[c]);
+    if (seg == 0 && p.dh0) store_turned<Sh>(p.dh0 + own + c * S, q, order, gc[c]);
   }
 }
 
 template <typename T, int S, bool VEC>
-__global__ void __launch_bounds__(BwdShape<S>::NT, BwdRegs<T, S>::CTAS) scan_bwd_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(BwdShape<S>::NT, BwdRegs<S>::CTAS) scan_bwd_kernel(const ScanParams p) {
   extern __shared__ __align__(16) unsigned char raw_smem[];
   BwdSmem<S>& sm = *reinterpret_cast<BwdSmem<S>*>(raw_smem);
   if (threadIdx.x >= BwdShape<S>::WALK) {
-    fewer_registers<BwdRegs<T, S>::LOADERS>();
+    fewer_registers<BwdRegs<S>::LOADERS>();
     scan_bwd_load<T, S, VEC>(p, sm);
   } else {
-    more_registers<BwdRegs<T, S>::WALKERS>();
+    more_registers<BwdRegs<S>::WALKERS>();
     scan_bwd_walk<T, S, VEC>(p, sm);
   }
 }
@@ -490,9 +549,9 @@ __global__ void __launch_bounds__(BwdShape<S>::NT, BwdRegs<T, S>::CTAS) scan_bwd
 // What a piece of the time axis adds to the gradient of the state in front of it (from zero behind it), and the product of its
 // decays, for pieces 1 .. nseg - 1.
 template <typename T, int S, bool VEC>
-__global__ void __launch_bounds__(BwdShape<S>::NT) scan_bwd_carry_kernel(const ScanParams p) {
-  using Sh = BwdShape<S>;
-  constexpr int TT = SCAN_TILE, CH = Sh::CH, C = Sh::C, NP = Sh::NP, NL = Sh::NL, NQ = Sh::NQ;
+__global__ void __launch_bounds__(BwdCarryShape<S>::NT) scan_bwd_carry_kernel(const ScanParams p) {
+  using Sh = BwdCarryShape<S>;
+  constexpr int TT = Sh::TT, CH = Sh::CH, C = Sh::C, NP = Sh::NP, NL = Sh::NL, NQ = Sh::NQ;
   __shared__ __align__(16) float2 dg[2][TT][CH];        // Delta, dy'
   __shared__ __align__(16) float cs[2][TT][S];
   const Place<CH> at(p, blockIdx.x);
@@ -668,19 +727,17 @@ template <typename T, int S, bool VEC>
 cudaError_t launch(const ScanParams& p, cudaStream_t s) {
   const unsigned grid = (unsigned)blocks_of(p, BwdShape<S>::CH);
   constexpr int smem = sizeof(BwdSmem<S>);
-  static unsigned long long raised = 0;      // devices whose limit is raised
-  if (smem > 48 * 1024) {
-    int dev = 0;
-    if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (!(__atomic_load_n(&raised, __ATOMIC_ACQUIRE) & bit)) {
-      const cudaError_t e = cudaFuncSetAttribute(scan_bwd_kernel<T, S, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      if (e != cudaSuccess) return e;
-      __atomic_fetch_or(&raised, bit, __ATOMIC_RELEASE);
-    }
+  static unsigned long long raised = 0;
+  static int registers = 0;      // of a thread at launch: the kernel shares them out
+  if (__atomic_load_n(&registers, __ATOMIC_RELAXED) == 0) {
+    cudaFuncAttributes a;
+    if (const cudaError_t e = cudaFuncGetAttributes(&a, scan_bwd_kernel<T, S, VEC>); e != cudaSuccess) return e;
+    if (a.numRegs * BwdShape<S>::NT < BwdRegs<S>::ALL) return cudaErrorLaunchOutOfResources;
+    __atomic_store_n(&registers, a.numRegs, __ATOMIC_RELAXED);
   }
+  if (const cudaError_t e = allow_smem(scan_bwd_kernel<T, S, VEC>, smem, &raised); e != cudaSuccess) return e;
   if (p.nseg > 1) {
-    scan_bwd_carry_kernel<T, S, VEC><<<dim3(grid, p.nseg - 1), BwdShape<S>::NT, 0, s>>>(p);
+    scan_bwd_carry_kernel<T, S, VEC><<<dim3(grid, p.nseg - 1), BwdCarryShape<S>::NT, 0, s>>>(p);
     if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   }
   scan_bwd_kernel<T, S, VEC><<<dim3(grid, p.nseg), BwdShape<S>::NT, smem, s>>>(p);
@@ -691,8 +748,6 @@ cudaError_t launch(const ScanParams& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 }  // namespace
-
-int scan_bwd_segments(int N, int L, int D, int sms) { return scan_segments(N, L, D, sms); }
 
 long long scan_bwd_scratch(ScanParams& p, float* base) {
   const long long ch = scan_bwd_channels(p.S), per = (p.D / p.G + ch - 1) / ch, slots = (long long)p.N * p.nseg;

@@ -9,16 +9,25 @@ namespace srwm {
 namespace {
 using namespace scan;
 
+template <typename Sh, bool CARRY>
+struct FwdSmem {
+  float2 dd[2][Sh::TT][Sh::CH];                                            // Delta, Delta u
+  float bc[2][CARRY ? 1 : 2][Sh::TT][Sh::S];
+  float ys[CARRY ? 1 : 2][CARRY ? 1 : Sh::TT][CARRY ? 1 : Sh::LN][Sh::PAD];   // C . h, a row of each lane of a channel
+};
+
 // CARRY: only what a piece of the time axis makes of the state (its end from zero, and the product of its decays), for the
 // pieces behind it; one CTA per 32 channels and piece.  Four warps load and prepare a tile, and write
 // the one before it, while the others walk the tile between: one barrier a tile.
 template <typename T, int S, bool VEC, int C, bool CARRY>
-__global__ void __launch_bounds__(Shape<S, C>::NT, S == 64 ? 1 : 2) scan_fwd_kernel(const ScanParams p) {
-  using Sh = Shape<S, C>;
-  constexpr int TT = SCAN_TILE, CH = Sh::CH, PAD = CH + 8, NP = Sh::NP, NL = Sh::NL, NQ = Sh::NQ, BUFS = CARRY ? 1 : 2;
-  __shared__ __align__(16) float2 dd[2][TT][CH];     // Delta, Delta u
-  __shared__ __align__(16) float bc[2][BUFS][TT][S];
-  __shared__ __align__(16) float ys[BUFS][TT][PAD];
+__global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 ? 1 : 2) scan_fwd_kernel(const ScanParams p) {
+  using Sh = Shape<S, C, SCAN_TILE>;
+  constexpr int TT = SCAN_TILE, CH = Sh::CH, NP = Sh::NP, NL = Sh::NL, NQ = Sh::NQ, BUFS = CARRY ? 1 : 2;
+  extern __shared__ __align__(16) unsigned char raw_smem[];
+  FwdSmem<Sh, CARRY>& sm = *reinterpret_cast<FwdSmem<Sh, CARRY>*>(raw_smem);
+  auto& dd = sm.dd;
+  auto& bc = sm.bc;
+  auto& ys = sm.ys;
   const Place<CH> at(p, blockIdx.x);
   const int seg = blockIdx.y, t_first = seg * p.seglen, t_end = min(p.L, t_first + p.seglen);
   if (threadIdx.x >= Sh::WALK) {
@@ -99,7 +108,7 @@ __global__ void __launch_bounds__(Shape<S, C>::NT, S == 64 ? 1 : 2) scan_fwd_ker
     for (int k = 0; k < NL; ++k) {
       const int t = t0 + row[k], v = t < t_end ? valid[k] : 0;
       if (v <= 0) continue;
-      const float4 s4 = *reinterpret_cast<const float4*>(&ys[buf][row[k]][col[k]]), u4 = u0[k].get();
+      const float4 s4 = sum_lanes<Sh>(&ys[buf][row[k]][0][col[k]]), u4 = u0[k].get();
       float4 y4 = make_float4(fmaf(skip[k].x, u4.x, s4.x), fmaf(skip[k].y, u4.y, s4.y), fmaf(skip[k].z, u4.z, s4.z), fmaf(skip[k].w, u4.w, s4.w));
       if (gate) {
         const float4 z4 = z0[k].get();
@@ -208,12 +217,11 @@ __global__ void __launch_bounds__(Shape<S, C>::NT, S == 64 ? 1 : 2) scan_fwd_ker
           }
         }
       };
-      float yv[C][Sh::LN];
       ahead(0, 0);
 #pragma unroll
       for (int t1 = 0; t1 < TT; t1 += PU) {
         const int b = t1 / PU % 2;
-        if (!WHOLE && t1 % Sh::LN == 0 && t1 >= steps) break;      // (what is summed over the lanes, LN steps at a time, is summed whole)
+        if (!WHOLE && t1 >= steps) break;
         if (t1 + PU < TT) ahead(t1 + PU, b ^ 1);
 #pragma unroll
         for (int k = 0; k < PU; ++k) {
@@ -226,6 +234,7 @@ __global__ void __launch_bounds__(Shape<S, C>::NT, S == 64 ? 1 : 2) scan_fwd_ker
           }
           const bool fresh = !WHOLE && (now >> t & 1u);
           if (CARRY && fresh) cut = true;
+          float y[C];
 #pragma unroll
           for (int c = 0; c < C; ++c) {
             u64 acc = 0ull;
@@ -235,16 +244,9 @@ __global__ void __launch_bounds__(Shape<S, C>::NT, S == 64 ? 1 : 2) scan_fwd_ker
               h[c][i] = WHOLE || t < steps ? next : h[c][i];
               if (!CARRY) acc = i == 0 ? mul2(h[c][i], c2[b][k][i]) : fma2<true>(h[c][i], c2[b][k][i], acc);
             }
-            yv[c][t % Sh::LN] = hsum2(acc);
+            y[c] = hsum2(acc);
           }
-          if (!CARRY && t % Sh::LN == Sh::LN - 1) {
-            float s[C];
-#pragma unroll
-            for (int c = 0; c < C; ++c) s[c] = steps_to_lanes<Sh::LN>(yv[c], q);
-            float* o = &ys[CARRY ? 0 : k0][t - (Sh::LN - 1) + q][chl];
-            if (C == 2) *reinterpret_cast<float2*>(o) = make_float2(s[0], s[C - 1]);
-            else *o = s[0];
-          }
+          if (!CARRY) store_channels<C>(&ys[CARRY ? 0 : k0][CARRY ? 0 : t][CARRY ? 0 : q][chl], y);
         }
       }
     };
@@ -272,8 +274,8 @@ __global__ void __launch_bounds__(Shape<S, C>::NT, S == 64 ? 1 : 2) scan_fwd_ker
 // bytes, and by its launch where these are few.  NB: sequences of a thread, whose loads are all on their way before the first is used; more
 // than one where there are enough of them (256 sequences x 2048 channels, S 16, bf16: 34 us with one, see the rule).
 template <typename T, int S, bool VEC, int NB>
-__global__ void __launch_bounds__(Shape<S, 1>::WALK) scan_step_kernel(const ScanParams p) {
-  using Sh = Shape<S, 1>;
+__global__ void __launch_bounds__(Shape<S, 1, SCAN_TILE>::WALK) scan_step_kernel(const ScanParams p) {
+  using Sh = Shape<S, 1, SCAN_TILE>;
   constexpr int NP = Sh::NP;
   chained();
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, q = lane % Sh::LN, chl = warp * Sh::LC + lane / Sh::LN;
@@ -343,37 +345,43 @@ __global__ void __launch_bounds__(Shape<S, 1>::WALK) scan_step_kernel(const Scan
 
 template <typename T, int S, bool VEC, int C>
 cudaError_t sequences(const ScanParams& p, cudaStream_t s) {
-  const unsigned grid = (unsigned)blocks_of(p, Shape<S, C>::CH);
+  using Sh = Shape<S, C, SCAN_TILE>;
+  const unsigned grid = (unsigned)blocks_of(p, Sh::CH);
+  static unsigned long long raised[2] = {0, 0};
   if (p.nseg > 1) {
-    scan_fwd_kernel<T, S, VEC, C, true><<<dim3(grid, p.nseg - 1), Shape<S, C>::NT, 0, s>>>(p);
+    constexpr int smem = sizeof(FwdSmem<Sh, true>);
+    if (const cudaError_t e = allow_smem(scan_fwd_kernel<T, S, VEC, C, true>, smem, &raised[0]); e != cudaSuccess) return e;
+    scan_fwd_kernel<T, S, VEC, C, true><<<dim3(grid, p.nseg - 1), Sh::NT, smem, s>>>(p);
     if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   }
-  scan_fwd_kernel<T, S, VEC, C, false><<<dim3(grid, p.nseg), Shape<S, C>::NT, 0, s>>>(p);
+  constexpr int smem = sizeof(FwdSmem<Sh, false>);
+  if (const cudaError_t e = allow_smem(scan_fwd_kernel<T, S, VEC, C, false>, smem, &raised[1]); e != cudaSuccess) return e;
+  scan_fwd_kernel<T, S, VEC, C, false><<<dim3(grid, p.nseg), Sh::NT, smem, s>>>(p);
   return cudaGetLastError();
 }
 template <typename T, int S, bool VEC>
 cudaError_t launch(const ScanParams& p, cudaStream_t s) {
   if (p.L <= SCAN_STEPS_DIRECT && !p.ckpt) {
     constexpr int NB = S <= 16 ? 4 : 2;
-    const long long grid = blocks_of(p, Shape<S, 1>::CH);
-    if (grid < 32 * common_sms()) return launch_behind(scan_step_kernel<T, S, VEC, 1>, p, dim3((unsigned)grid), Shape<S, 1>::WALK, 0, s);
-    return launch_behind(scan_step_kernel<T, S, VEC, NB>, p, dim3((unsigned)(grid / p.N * ((p.N + NB - 1) / NB))), Shape<S, 1>::WALK, 0, s);
+    const long long grid = blocks_of(p, Shape<S, 1, SCAN_TILE>::CH);
+    if (grid < 32 * common_sms()) return launch_behind(scan_step_kernel<T, S, VEC, 1>, p, dim3((unsigned)grid), Shape<S, 1, SCAN_TILE>::WALK, 0, s);
+    return launch_behind(scan_step_kernel<T, S, VEC, NB>, p, dim3((unsigned)(grid / p.N * ((p.N + NB - 1) / NB))), Shape<S, 1, SCAN_TILE>::WALK, 0, s);
   }
   // two channels a thread where these CTAs still fill the multiprocessors
   if constexpr (S > 8)
-    if (blocks_of(p, Shape<S, 2>::CH) * p.nseg >= 1 * common_sms()) return sequences<T, S, VEC, 2>(p, s);
+    if (blocks_of(p, Shape<S, 2, SCAN_TILE>::CH) * p.nseg >= 1 * common_sms()) return sequences<T, S, VEC, 2>(p, s);
   return sequences<T, S, VEC, 1>(p, s);
 }
 
 }  // namespace
 
-// One piece where the channels alone give every scheduler a warp; otherwise enough pieces for two, of 64 steps at least (a piece's
-// exponentials are formed twice).
-int scan_segments(int N, int L, int D, int sms) {
-  const long long ctas = (long long)N * ((D + 31) / 32);
-  if (ctas >= sms || L < 128) return 1;
-  long long n = (2 * sms + ctas - 1) / ctas;
-  if (n > L / 64) n = L / 64;
+// The pieces of the time axis.  One where the channels alone come near to filling the GPU; otherwise as many as fill it once, of 64 steps at
+// least.  A piece's exponentials are formed twice, so two pieces gain nothing.
+int scan_segments(const ScanParams& p, int channels, int sms) {
+  const long long ctas = blocks_of(p, channels), room = (long long)sms * (p.S == 64 ? 1 : 2);
+  if (ctas == 0 || p.L < 192) return 1;
+  long long n = room / ctas;
+  if (n > p.L / 64) n = p.L / 64;
   if (n > 64) n = 64;
   return n < 3 ? 1 : (int)n;
 }

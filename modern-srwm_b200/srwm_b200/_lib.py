@@ -201,7 +201,7 @@ SYMBOLS = {
     "srwm_b200_scan_forward": (C.c_int, [C.POINTER(ScanArgs), C.c_void_p]),
     "srwm_b200_scan_backward": (C.c_int, [C.POINTER(ScanArgs), C.POINTER(ScanGrads), C.c_void_p]),
     "srwm_b200_scan_checkpoint_floats": (C.c_int64, [C.c_int32] * 4),
-    "srwm_b200_scan_scratch_bytes": (C.c_int64, [C.c_int32] * 4),
+    "srwm_b200_scan_scratch_bytes": (C.c_int64, [C.c_int32] * 5),
     "srwm_b200_scan_backward_scratch_bytes": (C.c_int64, [C.c_int32] * 5),
     "srwm_b200_conv_forward": (C.c_int, [C.POINTER(ConvArgs), C.c_void_p]),
     "srwm_b200_conv_backward": (C.c_int, [C.POINTER(ConvArgs), C.POINTER(ConvGrads), C.c_void_p]),

@@ -63,8 +63,8 @@ def test_scan_refusals():
     assert f(C.byref(_scan_args(N=1 << 20, D=1 << 20)), None) == L.ERR_SHAPE
     assert f(C.byref(_scan_args(N=0)), None) == 0 and f(C.byref(_scan_args(D=0)), None) == 0
     # a long time axis of few channels is cut into pieces, which need scratch
-    assert L.load().srwm_b200_scan_scratch_bytes(1, 4096, 64, 16) > 0
-    assert L.load().srwm_b200_scan_scratch_bytes(64, 4096, 2048, 16) == 0
+    assert L.load().srwm_b200_scan_scratch_bytes(1, 4096, 64, 16, 1) > 0
+    assert L.load().srwm_b200_scan_scratch_bytes(64, 4096, 2048, 16, 2) == 0
     assert f(C.byref(_scan_args(N=1, L=4096)), None) == L.ERR_NULL
     g, grads = L.load().srwm_b200_scan_backward, L.ScanGrads()
     assert g(C.byref(_scan_args()), None, None) == L.ERR_NULL
