@@ -150,16 +150,55 @@ __device__ __forceinline__ void put4(__nv_bfloat16* p, int valid, float4 v) {
   }
 }
 
+// Four values as two pairs
+struct Pairs {
+  u64 lo, hi;
+  __device__ __forceinline__ Pairs() : lo(0ull), hi(0ull) {}
+  __device__ __forceinline__ Pairs(u64 a, u64 b) : lo(a), hi(b) {}
+  __device__ __forceinline__ explicit Pairs(float4 v) : lo(pack2(v.x, v.y)), hi(pack2(v.z, v.w)) {}
+  __device__ __forceinline__ explicit Pairs(const float* p) {
+    const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(p);
+    lo = t.x;
+    hi = t.y;
+  }
+  __device__ __forceinline__ float4 f4() const {
+    float4 v;
+    unpack2(lo, v.x, v.y);
+    unpack2(hi, v.z, v.w);
+    return v;
+  }
+};
+__device__ __forceinline__ Pairs operator+(Pairs a, Pairs b) { return Pairs(add2(a.lo, b.lo), add2(a.hi, b.hi)); }
+__device__ __forceinline__ Pairs operator*(Pairs a, Pairs b) { return Pairs(mul2(a.lo, b.lo), mul2(a.hi, b.hi)); }
+__device__ __forceinline__ Pairs fma4(Pairs a, Pairs b, Pairs c) { return Pairs(fma2<true>(a.lo, b.lo, c.lo), fma2<true>(a.hi, b.hi, c.hi)); }
+__device__ __forceinline__ Pairs softplus4(Pairs x) { return Pairs(softplus2(x.lo), softplus2(x.hi)); }
+__device__ __forceinline__ Pairs sigmoid4(Pairs x) {
+  const float4 v = x.f4();
+  return Pairs(make_float4(sigmoid(v.x), sigmoid(v.y), sigmoid(v.z), sigmoid(v.w)));
+}
 // The same step's values of the LN lanes' rows, added up
 template <typename Sh>
-__device__ __forceinline__ float4 sum_lanes(const float* p) {
-  float4 v = *reinterpret_cast<const float4*>(p);
+__device__ __forceinline__ Pairs sum_lanes(const float* p) {
+  Pairs v(p);
 #pragma unroll
-  for (int q = 1; q < Sh::LN; ++q) {
-    const float4 o = *reinterpret_cast<const float4*>(p + q * Sh::PAD);
-    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-  }
+  for (int q = 1; q < Sh::LN; ++q) v = v + Pairs(p + q * Sh::PAD);
   return v;
+}
+// Delta and Delta u of four channels side by side
+__device__ __forceinline__ void store_staged(float2* p, Pairs a, Pairs b) {
+  const float4 x = a.f4(), y = b.f4();
+  reinterpret_cast<float4*>(p)[0] = make_float4(x.x, y.x, x.y, y.y);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x.z, y.z, x.w, y.w);
+}
+// Four of a vector over the channels
+__device__ __forceinline__ Pairs four(const float* p, int valid) {
+  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p == nullptr) return Pairs(r);
+  if (valid > 0) r.x = p[0];
+  if (valid > 1) r.y = p[1];
+  if (valid > 2) r.z = p[2];
+  if (valid > 3) r.w = p[3];
+  return Pairs(r);
 }
 template <int C>
 __device__ __forceinline__ void store_channels(float* p, const float* v) {

@@ -136,65 +136,60 @@ __device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& s
 #pragma unroll
     for (int k = 0; k < NL; ++k) sm.sums[0][tid + k * Sh::LOAD] = sm.sums[1][tid + k * Sh::LOAD] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  auto place = [&](const ScanRows& w, int t) { return reinterpret_cast<T*>(w.p) + at.n * w.sn + t * w.sl + at.ch0 + col; };
-  float bias[4], skip[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    bias[i] = i < valid && p.bias ? p.bias[at.ch0 + col + i] : 0.f;
-    skip[i] = i < valid && p.skip ? p.skip[at.ch0 + col + i] : 0.f;
-  }
-  Quad<T, VEC> fu[NL], fd[NL], fz[NL], fy[NL], fb[NQ], fc[NQ];
-  auto fetch_rows = [&](int t0) {
+  // (each pointer walks with its tiles, the last first: the loads' two tiles in front of the results')
+  auto place = [&](const ScanRows& w) { return reinterpret_cast<T*>(w.p) + at.n * w.sn + (t_last + row) * w.sl + at.ch0 + col; };
+  const T *pu = place(p.u), *pd = place(p.delta), *pz = place(p.z), *py = place(p.dy);
+  T *ou = place(p.du), *od = place(p.ddelta), *oz = place(p.dz);
+  const int id0 = tid % Sh::QUADS, bc_row = tid < Sh::QUADS ? id0 / (S / 4) : p.L;      // (a row behind every piece's end)
+  const T* pb = reinterpret_cast<const T*>(p.B.p) + at.n * p.B.sn + at.g * p.B.sg + (t_last + id0 / (S / 4)) * p.B.sl + id0 % (S / 4) * 4;
+  const T* pc = reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + (t_last + id0 / (S / 4)) * p.C.sl + id0 % (S / 4) * 4;
+  static_assert(NQ == 1, "a tile's B is a piece a thread");
+  const Pairs bias = four(p.bias ? p.bias + at.ch0 + col : nullptr, valid), skip = four(p.skip ? p.skip + at.ch0 + col : nullptr, valid);
+  // three tiles: being fetched, staged for the next walk, walked before (these two for the results; where they take more than 16
+  // registers, the rows are loaded again instead)
+  constexpr bool KEEP = VEC && NL * sizeof(T) == 2;
+  struct Rows {
+    Quad<T, VEC> u, d, z, y;
+  } next[NL], staged[KEEP ? NL : 1], done[KEEP ? NL : 1];
+  Quad<T, VEC> fb, fc;
+  auto fetch = [&](int t0) {
 #pragma unroll
     for (int k = 0; k < NL; ++k) {
-      const int t = t0 + row + k * RS, v = t < t_end ? valid : 0;
-      fu[k].fetch(place(p.u, t), v);
-      fd[k].fetch(place(p.delta, t), v);
-      fy[k].fetch(place(p.dy, t), v);
-      if (gate) fz[k].fetch(place(p.z, t), v);
+      const int v = t0 + row + k * RS < t_end ? valid : 0;
+      next[k].u.fetch(pu + k * RS * p.u.sl, v);
+      next[k].d.fetch(pd + k * RS * p.delta.sl, v);
+      next[k].y.fetch(py + k * RS * p.dy.sl, v);
+      if (gate) next[k].z.fetch(pz + k * RS * p.z.sl, v);
     }
-  };
-  auto fetch_bc = [&](int t0) {
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int id = tid + i * Sh::LOAD, c = id % (S / 4) * 4, t = t0 + id / (S / 4), v = id < Sh::QUADS && t < t_end ? 4 : 0;
-      fb[i].fetch(reinterpret_cast<const T*>(p.B.p) + at.n * p.B.sn + at.g * p.B.sg + t * p.B.sl + c, v);
-      fc[i].fetch(reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + t * p.C.sl + c, v);
-    }
+    pu -= TT * p.u.sl; pd -= TT * p.delta.sl; py -= TT * p.dy.sl; pz -= TT * p.z.sl;
+    const int v = t0 + bc_row < t_end ? 4 : 0;
+    fb.fetch(pb, v);
+    fc.fetch(pc, v);
+    pb -= TT * p.B.sl; pc -= TT * p.C.sl;
   };
   auto stage = [&](int buf) {
     auto& tl = sm.tile[buf];
 #pragma unroll
     for (int k = 0; k < NL; ++k) {
-      if (!loads) break;
-      const float4 u4 = fu[k].get(), r4 = fd[k].get();
-      u64 lo = add2(pack2(r4.x, r4.y), pack2(bias[0], bias[1])), hi = add2(pack2(r4.z, r4.w), pack2(bias[2], bias[3]));
-      if (p.softplus) {
-        lo = softplus2(lo);
-        hi = softplus2(hi);
+      if (KEEP) {
+        done[KEEP ? k : 0] = staged[KEEP ? k : 0];
+        staged[KEEP ? k : 0] = next[k];
       }
-      const u64 xlo = mul2(lo, pack2(u4.x, u4.y)), xhi = mul2(hi, pack2(u4.z, u4.w));
-      float dl[4], du[4];
-      float4 g = fy[k].get();
-      unpack2(lo, dl[0], dl[1]); unpack2(hi, dl[2], dl[3]);
-      unpack2(xlo, du[0], du[1]); unpack2(xhi, du[2], du[3]);
+      if (!loads) continue;
+      Pairs dl = Pairs(next[k].d.get()) + bias, g(next[k].y.get());
+      if (p.softplus) dl = softplus4(dl);
       if (gate) {
-        const float4 z4 = fz[k].get();
-        g.x *= z4.x * sigmoid(z4.x); g.y *= z4.y * sigmoid(z4.y); g.z *= z4.z * sigmoid(z4.z); g.w *= z4.w * sigmoid(z4.w);
+        const Pairs z(next[k].z.get());
+        g = g * (z * sigmoid4(z));
       }
-      float4* o = reinterpret_cast<float4*>(&tl.dd[row + k * RS][col]);
-      o[0] = make_float4(dl[0], du[0], dl[1], du[1]);
-      o[1] = make_float4(dl[2], du[2], dl[3], du[3]);
-      *reinterpret_cast<float4*>(&tl.gy[row + k * RS][col]) = g;
+      store_staged(&tl.dd[row + k * RS][col], dl, dl * Pairs(next[k].u.get()));
+      *reinterpret_cast<float4*>(&tl.gy[row + k * RS][col]) = g.f4();
     }
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int id = tid + i * Sh::LOAD, c = id % (S / 4) * 4, r = id / (S / 4);
-      if (id >= Sh::QUADS) continue;
+    if (tid < Sh::QUADS) {
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        const float4 v = w ? fc[i].get() : fb[i].get();
-        float* o = &tl.bc[w][r][0][c];
+        const float4 v = w ? fc.get() : fb.get();
+        float* o = &tl.bc[w][id0 / (S / 4)][0][id0 % (S / 4) * 4];
         *reinterpret_cast<float4*>(o) = v;
         *reinterpret_cast<float4*>(o + S) = make_float4(v.z, v.w, v.x, v.y);
         *reinterpret_cast<float4*>(o + 2 * S) = make_float4(v.y, v.x, v.w, v.z);
@@ -202,82 +197,69 @@ __device__ __forceinline__ void scan_bwd_load(const ScanParams& p, BwdSmem<S>& s
       }
     }
   };
+  float* part = p.part_bc + ((long long)at.blk * 2 * p.N + at.n) * p.L * p.G * S + at.g * S;
   auto finish = [&](int t0, int buf) {
     const auto& tl = sm.tile[buf];
     const int steps = min(TT, t_end - t0);
     // this CTA's share of dB and dC
-#pragma unroll 1
-    for (int e = tid; e < steps * 2 * S / 4; e += Sh::LOAD) {
-      const int s = e % (S / 4) * 4, arr = e / (S / 4) % 2, t = e / (S / 2);
-      float4 v = *reinterpret_cast<const float4*>(&tl.part[0][t][arr][s]);
 #pragma unroll
-      for (int w = 1; w < Sh::WARPS; ++w) {
-        const float4 o = *reinterpret_cast<const float4*>(&tl.part[w][t][arr][s]);
-        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-      }
-      *reinterpret_cast<float4*>(p.part_bc + ((((long long)at.blk * 2 + arr) * p.N + at.n) * p.L + t0 + t) * p.G * S + at.g * S + s) = v;
+    for (int e0 = 0; e0 < 2 * Sh::QUADS; e0 += Sh::LOAD) {
+      const int e = e0 + tid, s = e % (S / 4) * 4, arr = e / (S / 4) % 2, t = e / (S / 2);
+      if (e >= 2 * Sh::QUADS || t >= steps) continue;
+      Pairs v(&tl.part[0][t][arr][s]);
+#pragma unroll
+      for (int w = 1; w < Sh::WARPS; ++w) v = v + Pairs(&tl.part[w][t][arr][s]);
+      *reinterpret_cast<float4*>(part + ((long long)arr * p.N * p.L + t0 + t) * p.G * S + s) = v.f4();
     }
-    // (the tile's rows again: they have left the registers)
-#pragma unroll 1
+#pragma unroll
     for (int k = 0; k < NL; ++k) {
-      const int r = row + k * RS, t = t0 + r, v = r < steps ? valid : 0;
-      if (v <= 0) break;
-      Quad<T, VEC> q0, q1, q2, q3;
-      q0.fetch(place(p.u, t), v);
-      q1.fetch(place(p.delta, t), v);
-      if (gate) {
-        q2.fetch(place(p.z, t), v);
-        q3.fetch(place(p.dy, t), v);
-      }
-      const float4 gb4 = sum_lanes<Sh>(&tl.gb[r][0][col]), sa4 = sum_lanes<Sh>(&tl.sa[r][0][col]);
-      const float4 g4 = *reinterpret_cast<const float4*>(&tl.gy[r][col]);
-      const float4* dk = reinterpret_cast<const float4*>(&tl.dd[r][col]);
-      const float4 d01 = dk[0], d23 = dk[1], u4 = q0.get(), r4 = q1.get();
-      const float dl[4] = {d01.x, d01.z, d23.x, d23.z}, us[4] = {u4.x, u4.y, u4.z, u4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w};
-      const float rs[4] = {r4.x, r4.y, r4.z, r4.w}, gb[4] = {gb4.x, gb4.y, gb4.z, gb4.w}, sa[4] = {sa4.x, sa4.y, sa4.z, sa4.w};
-      float o1[4], o2[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o1[i] = fmaf(g[i], skip[i], dl[i] * gb[i]);
-        o2[i] = fmaf(us[i], gb[i], sa[i] * 0.6931471805599453f);      // (the walking threads' A has log2(e) in it)
-        if (p.softplus) o2[i] *= sigmoid(rs[i] + bias[i]);
-      }
-      put4<VEC>(place(p.du, t), v, make_float4(o1[0], o1[1], o1[2], o1[3]));
-      put4<VEC>(place(p.ddelta, t), v, make_float4(o2[0], o2[1], o2[2], o2[3]));
-      const int id = tid + k * Sh::LOAD;
-      float4 w = sm.sums[0][id];
-      sm.sums[0][id] = make_float4(fmaf(g[0], us[0], w.x), fmaf(g[1], us[1], w.y), fmaf(g[2], us[2], w.z), fmaf(g[3], us[3], w.w));
-      w = sm.sums[1][id];
-      sm.sums[1][id] = make_float4(w.x + o2[0], w.y + o2[1], w.z + o2[2], w.w + o2[3]);
-      if (gate) {
-        const float4 yp4 = sum_lanes<Sh>(&tl.yp[r][0][col]), z4 = q2.get(), y4 = q3.get();
-        const float yp[4] = {yp4.x, yp4.y, yp4.z, yp4.w}, zs[4] = {z4.x, z4.y, z4.z, z4.w}, os[4] = {y4.x, y4.y, y4.z, y4.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float sg = sigmoid(zs[i]);
-          o1[i] = os[i] * fmaf(skip[i], us[i], yp[i]) * sg * fmaf(zs[i], 1.f - sg, 1.f);
+      const int r = row + k * RS, v = r < steps ? valid : 0;
+      if (v > 0) {
+        Rows was = done[KEEP ? k : 0];
+        if (!KEEP) {
+          const int t = t0 - t_last + k * RS;      // (the pointers at the last tile, from the results')
+          was.u.fetch(place(p.u) + t * p.u.sl, v);
+          was.d.fetch(place(p.delta) + t * p.delta.sl, v);
+          if (gate) {
+            was.z.fetch(place(p.z) + t * p.z.sl, v);
+            was.y.fetch(place(p.dy) + t * p.dy.sl, v);
+          }
         }
-        put4<VEC>(place(p.dz, t), v, make_float4(o1[0], o1[1], o1[2], o1[3]));
+        const Pairs g(&tl.gy[r][col]), u(was.u.get()), gb = sum_lanes<Sh>(&tl.gb[r][0][col]), sa = sum_lanes<Sh>(&tl.sa[r][0][col]);
+        const float4* dk = reinterpret_cast<const float4*>(&tl.dd[r][col]);
+        const float4 d01 = dk[0], d23 = dk[1];
+        const Pairs dl(make_float4(d01.x, d01.z, d23.x, d23.z));
+        put4<VEC>(ou + k * RS * p.du.sl, v, fma4(g, skip, dl * gb).f4());
+        const u64 ln2 = dup2(0.6931471805599453f);      // (the walking threads' A has log2(e) in it)
+        Pairs dr = fma4(u, gb, sa * Pairs(ln2, ln2));
+        if (p.softplus) dr = dr * sigmoid4(Pairs(was.d.get()) + bias);
+        put4<VEC>(od + k * RS * p.ddelta.sl, v, dr.f4());
+        const int id = tid + k * Sh::LOAD;
+        sm.sums[0][id] = fma4(g, u, Pairs(sm.sums[0][id])).f4();
+        sm.sums[1][id] = (Pairs(sm.sums[1][id]) + dr).f4();
+        if (gate) {      // silu'(z) = sigmoid (1 + z (1 - sigmoid))
+          const u64 one = dup2(1.f), minus = dup2(-1.f);
+          const Pairs y = fma4(skip, u, sum_lanes<Sh>(&tl.yp[r][0][col])), z(was.z.get()), sg = sigmoid4(z);
+          const Pairs rest = fma4(sg, Pairs(minus, minus), Pairs(one, one));
+          put4<VEC>(oz + k * RS * p.dz.sl, v, (Pairs(was.y.get()) * y * (sg * fma4(z, rest, Pairs(one, one)))).f4());
+        }
       }
     }
+    ou -= TT * p.du.sl; od -= TT * p.ddelta.sl; oz -= TT * p.dz.sl;
   };
-  fetch_rows(t_last);
-  fetch_bc(t_last);
+  fetch(t_last);
   stage(0);
-  if (t_last - TT >= t_first) {
-    fetch_rows(t_last - TT);
-    fetch_bc(t_last - TT);
-  }
+  if (t_last - TT >= t_first) fetch(t_last - TT);
   __syncthreads();
   int k0 = 0;
   for (int t0 = t_last; t0 >= t_first; t0 -= TT, k0 ^= 1) {
     if (t0 < t_last) finish(t0 + TT, k0 ^ 1);
     if (t0 - TT >= t_first) {
       stage(k0 ^ 1);
-      if (t0 - 2 * TT >= t_first) {
-        fetch_rows(t0 - 2 * TT);
-        fetch_bc(t0 - 2 * TT);
-      }
+      if (t0 - 2 * TT >= t_first) fetch(t0 - 2 * TT);
+    } else {
+#pragma unroll
+      for (int k = 0; k < (KEEP ? NL : 1); ++k) done[k] = staged[k];
     }
     __syncthreads();
   }
@@ -298,7 +280,7 @@ template <typename T, int S, bool VEC>
 __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& sm) {
   using Sh = BwdShape<S>;
   constexpr int TT = Sh::TT, CH = Sh::CH, C = Sh::C, NP = Sh::NP, ST = Sh::ST, LN = Sh::LN;
-  constexpr int SUB = 4, GS = 8 / ST;
+  constexpr int SUB = 4, GS = 8 / ST, HOLD = ST == 4 ? SUB : 1;      // HOLD: steps whose sums over the groups are formed together
   static_assert(TT == SCAN_CKPT && TT == 2 * SUB, "a tile's steps are those between two of the forward's states");
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, q = lane % LN, chl = (warp * Sh::LC + lane / LN) * C;
   const Place<CH> at(p, blockIdx.x);
@@ -380,6 +362,17 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
       }
     };
 
+    // HOLD steps' shares of dB or dC from t on
+    auto leave = [&](float* v, int t, int arr) __attribute__((always_inline)) {
+#pragma unroll
+      for (int g = 0; g < HOLD / GS; ++g) sum_groups<ST, LN>(v + 8 * g, lane);
+#pragma unroll
+      for (int g = 0; g < HOLD / GS; ++g) {
+        float* o = part_mine + ((t + g * GS) * 2 + arr) * S;
+        if (LN == 8) *reinterpret_cast<float2*>(o) = make_float2(v[8 * g], v[8 * g + 1]);
+        else if (keeps) *o = v[8 * g];
+      }
+    };
     // Four steps at a time, the last first.  The second four have the first four walked on the way to them (without what they leave), so that a
     // and a h of no more than four stay in registers.
     auto tile = [&](auto whole) __attribute__((always_inline)) {
@@ -436,11 +429,11 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
             }
           }
         }
-        float v8[8];
+        float v[HOLD * ST];
 #pragma unroll
         for (int k = 0; k < SUB; ++k) {
           const int t = s0 + k;
-          float* vk = v8 + k % GS * ST;
+          float* vk = v + k % HOLD * ST;
           if (WHOLE || t < steps) {
             const bool fresh = !WHOLE && (now >> t & 1u);
             u64 c2[NP], sum[NP];
@@ -468,17 +461,12 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
 #pragma unroll
             for (int i = 0; i < ST; ++i) vk[i] = 0.f;
           }
-          if (k % GS == GS - 1) {
-            sum_groups<ST, LN>(v8, lane);
-            float* o = part_mine + (t - (GS - 1)) * 2 * S + S;
-            if (LN == 8) *reinterpret_cast<float2*>(o) = make_float2(v8[0], v8[1]);
-            else if (keeps) *o = v8[0];
-          }
+          if (k % HOLD == HOLD - 1) leave(v, t - (HOLD - 1), 1);
         }
 #pragma unroll
         for (int k = SUB - 1; k >= 0; --k) {
           const int t = s0 + k;
-          float* vk = v8 + k % GS * ST;
+          float* vk = v + k % HOLD * ST;
           if (WHOLE || t < steps) {
             float2 x[C];
             load_channels<C>(&tl.dd[t][chl], x);
@@ -511,12 +499,7 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
 #pragma unroll
             for (int i = 0; i < ST; ++i) vk[i] = 0.f;
           }
-          if (k % GS == 0) {
-            sum_groups<ST, LN>(v8, lane);
-            float* o = part_mine + t * 2 * S;
-            if (LN == 8) *reinterpret_cast<float2*>(o) = make_float2(v8[0], v8[1]);
-            else if (keeps) *o = v8[0];
-          }
+          if (k % HOLD == 0) leave(v, t, 0);
         }
       }
     };

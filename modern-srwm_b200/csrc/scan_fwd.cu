@@ -31,117 +31,93 @@ __global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 ? 1 : 2) s
   const Place<CH> at(p, blockIdx.x);
   const int seg = blockIdx.y, t_first = seg * p.seglen, t_end = min(p.L, t_first + p.seglen);
   if (threadIdx.x >= Sh::WALK) {
-  const int tid = threadIdx.x - Sh::WALK;
-  // the pieces of a tile that this thread loads, and stores again
-  const bool gate = !CARRY && p.z.p != nullptr;
-  int row[NL], col[NL], valid[NL];
-#pragma unroll
-  for (int k = 0; k < NL; ++k) {
-    const int id = tid + k * Sh::LOAD;
-    row[k] = id / (CH / 4);
-    col[k] = id % (CH / 4) * 4;
-    valid[k] = max(0, min(4, at.left - col[k]));
-  }
-  auto place = [&](const ScanRows& w, int t, int k) { return reinterpret_cast<T*>(w.p) + at.n * w.sn + t * w.sl + at.ch0 + col[k]; };
-  // three tiles: being fetched, staged for the next walk (u and z stay for its result), walked before
-  Quad<T, VEC> fu[NL], fd[NL], fz[NL], fb[NQ], fc[NQ], u1[NL], z1[NL], u0[NL], z0[NL];
-  auto fetch = [&](int t0) {
-#pragma unroll
-    for (int k = 0; k < NL; ++k) {
-      const int t = t0 + row[k], v = t < t_end ? valid[k] : 0;
-      fu[k].fetch(place(p.u, t, k), v);
-      fd[k].fetch(place(p.delta, t, k), v);
-      if (gate) fz[k].fetch(place(p.z, t, k), v);
-    }
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int id = tid + i * Sh::LOAD, c = id % (S / 4) * 4, t = t0 + id / (S / 4), v = id < Sh::QUADS && t < t_end ? 4 : 0;
-      fb[i].fetch(reinterpret_cast<const T*>(p.B.p) + at.n * p.B.sn + at.g * p.B.sg + t * p.B.sl + c, v);
-      if (!CARRY) fc[i].fetch(reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + t * p.C.sl + c, v);
-    }
-  };
-  auto four = [&](const float* w, int k) {      // of a vector over the channels
-    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float* f = w + at.ch0 + col[k];
-    if (w == nullptr) return r;
-    if (valid[k] > 0) r.x = f[0];
-    if (valid[k] > 1) r.y = f[1];
-    if (valid[k] > 2) r.z = f[2];
-    if (valid[k] > 3) r.w = f[3];
-    return r;
-  };
-  float4 bias[NL], skip[NL];
-#pragma unroll
-  for (int k = 0; k < NL; ++k) {
-    bias[k] = four(p.bias, k);
-    if (!CARRY) skip[k] = four(p.skip, k);
-  }
-  auto stage = [&](int buf) {
-#pragma unroll
-    for (int k = 0; k < NL; ++k) {
-      u0[k] = u1[k]; z0[k] = z1[k];
-      u1[k] = fu[k]; z1[k] = fz[k];
-      const float4 u4 = fu[k].get(), r4 = fd[k].get();
-      u64 lo = add2(pack2(r4.x, r4.y), pack2(bias[k].x, bias[k].y)), hi = add2(pack2(r4.z, r4.w), pack2(bias[k].z, bias[k].w));
-      if (p.softplus) {
-        lo = softplus2(lo);
-        hi = softplus2(hi);
-      }
-      const u64 xlo = mul2(lo, pack2(u4.x, u4.y)), xhi = mul2(hi, pack2(u4.z, u4.w));
-      float dl[4], du[4];
-      unpack2(lo, dl[0], dl[1]); unpack2(hi, dl[2], dl[3]);
-      unpack2(xlo, du[0], du[1]); unpack2(xhi, du[2], du[3]);
-      float4* o = reinterpret_cast<float4*>(&dd[buf][row[k]][col[k]]);
-      o[0] = make_float4(dl[0], du[0], dl[1], du[1]);
-      o[1] = make_float4(dl[2], du[2], dl[3], du[3]);
-    }
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int id = tid + i * Sh::LOAD;
-      if (id >= Sh::QUADS) continue;
-      *reinterpret_cast<float4*>(&bc[buf][0][0][0] + id * 4) = fb[i].get();
-      if (!CARRY) *reinterpret_cast<float4*>(&bc[buf][BUFS - 1][0][0] + id * 4) = fc[i].get();
-    }
-  };
-  auto finish = [&](int t0, int buf) {      // y of the tile walked before
-#pragma unroll
-    for (int k = 0; k < NL; ++k) {
-      const int t = t0 + row[k], v = t < t_end ? valid[k] : 0;
-      if (v <= 0) continue;
-      const float4 s4 = sum_lanes<Sh>(&ys[buf][row[k]][0][col[k]]), u4 = u0[k].get();
-      float4 y4 = make_float4(fmaf(skip[k].x, u4.x, s4.x), fmaf(skip[k].y, u4.y, s4.y), fmaf(skip[k].z, u4.z, s4.z), fmaf(skip[k].w, u4.w, s4.w));
-      if (gate) {
-        const float4 z4 = z0[k].get();
-        y4.x *= z4.x * sigmoid(z4.x); y4.y *= z4.y * sigmoid(z4.y);
-        y4.z *= z4.z * sigmoid(z4.z); y4.w *= z4.w * sigmoid(z4.w);
-      }
-      put4<VEC>(place(p.y, t, k), v, y4);
-    }
-  };
-
-  if (t_first < t_end) {
-    fetch(t_first);
-    stage(0);
-    if (t_first + TT < t_end) fetch(t_first + TT);
-  }
-  __syncthreads();
-  int k0 = 0;
-  for (int t0 = t_first; t0 < t_end; t0 += TT, k0 ^= 1) {
-    if (!CARRY && t0 > t_first) finish(t0 - TT, k0 ^ 1);
-    if (t0 + TT < t_end) {
-      stage(k0 ^ 1);
-      if (t0 + 2 * TT < t_end) fetch(t0 + 2 * TT);
-    } else {
+    const int tid = threadIdx.x - Sh::WALK;
+    // the pieces of a tile that this thread loads, and stores again: the same four channels, RS rows apart
+    constexpr int RS = Sh::LOAD / (CH / 4);
+    static_assert(Sh::LOAD % (CH / 4) == 0 && Sh::PIECES % Sh::LOAD == 0, "a thread's pieces have the same columns");
+    const bool gate = !CARRY && p.z.p != nullptr;
+    const int row = tid / (CH / 4), col = tid % (CH / 4) * 4, valid = max(0, min(4, at.left - col));
+    auto place = [&](const ScanRows& w) { return reinterpret_cast<T*>(w.p) + at.n * w.sn + (t_first + row) * w.sl + at.ch0 + col; };
+    const T *pu = place(p.u), *pd = place(p.delta), *pz = place(p.z);
+    T* py = place(p.y);
+    const int id0 = tid % Sh::QUADS, bc_row = tid < Sh::QUADS ? id0 / (S / 4) : p.L;      // (a row behind every piece's end)
+    constexpr int RBC = Sh::LOAD / (S / 4);
+    const T* pb = reinterpret_cast<const T*>(p.B.p) + at.n * p.B.sn + at.g * p.B.sg + (t_first + id0 / (S / 4)) * p.B.sl + id0 % (S / 4) * 4;
+    const T* pc = reinterpret_cast<const T*>(p.C.p) + at.n * p.C.sn + at.g * p.C.sg + (t_first + id0 / (S / 4)) * p.C.sl + id0 % (S / 4) * 4;
+    const Pairs bias = four(p.bias ? p.bias + at.ch0 + col : nullptr, valid), skip = four(!CARRY && p.skip ? p.skip + at.ch0 + col : nullptr, valid);
+    // three tiles: being fetched, staged for the next walk (u and z stay for its result), walked before
+    Quad<T, VEC> fu[NL], fd[NL], fz[NL], fb[NQ], fc[NQ], u1[NL], z1[NL], u0[NL], z0[NL];
+    auto fetch = [&](int t0) {      // tiles are asked for in order
 #pragma unroll
       for (int k = 0; k < NL; ++k) {
-        u0[k] = u1[k];
-        z0[k] = z1[k];
+        const int v = t0 + row + k * RS < t_end ? valid : 0;
+        fu[k].fetch(pu + k * RS * p.u.sl, v);
+        fd[k].fetch(pd + k * RS * p.delta.sl, v);
+        if (gate) fz[k].fetch(pz + k * RS * p.z.sl, v);
       }
+      pu += TT * p.u.sl; pd += TT * p.delta.sl; pz += TT * p.z.sl;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const int v = t0 + bc_row + i * RBC < t_end ? 4 : 0;
+        fb[i].fetch(pb + i * RBC * p.B.sl, v);
+        if (!CARRY) fc[i].fetch(pc + i * RBC * p.C.sl, v);
+      }
+      pb += TT * p.B.sl; pc += TT * p.C.sl;
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+      for (int k = 0; k < NL; ++k) {
+        u0[k] = u1[k]; z0[k] = z1[k];
+        u1[k] = fu[k]; z1[k] = fz[k];
+        Pairs dl = Pairs(fd[k].get()) + bias;
+        if (p.softplus) dl = softplus4(dl);
+        store_staged(&dd[buf][row + k * RS][col], dl, dl * Pairs(fu[k].get()));
+      }
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        if (tid >= Sh::QUADS) continue;
+        *reinterpret_cast<float4*>(&bc[buf][0][0][0] + (tid + i * Sh::LOAD) * 4) = fb[i].get();
+        if (!CARRY) *reinterpret_cast<float4*>(&bc[buf][BUFS - 1][0][0] + (tid + i * Sh::LOAD) * 4) = fc[i].get();
+      }
+    };
+    auto finish = [&](int t0, int buf) {      // y of the tile walked before
+#pragma unroll
+      for (int k = 0; k < NL; ++k) {
+        const int v = t0 + row + k * RS < t_end ? valid : 0;
+        if (v > 0) {
+          Pairs y = fma4(skip, Pairs(u0[k].get()), sum_lanes<Sh>(&ys[buf][row + k * RS][0][col]));
+          if (gate) {
+            const Pairs z(z0[k].get());
+            y = y * (z * sigmoid4(z));
+          }
+          put4<VEC>(py + k * RS * p.y.sl, v, y.f4());
+        }
+      }
+      py += TT * p.y.sl;
+    };
+    if (t_first < t_end) {
+      fetch(t_first);
+      stage(0);
+      if (t_first + TT < t_end) fetch(t_first + TT);
     }
     __syncthreads();
-  }
-  if (!CARRY && t_first < t_end) finish(t_first + (t_end - t_first - 1) / TT * TT, k0 ^ 1);
-  return;
+    int k0 = 0;
+    for (int t0 = t_first; t0 < t_end; t0 += TT, k0 ^= 1) {
+      if (!CARRY && t0 > t_first) finish(t0 - TT, k0 ^ 1);
+      if (t0 + TT < t_end) {
+        stage(k0 ^ 1);
+        if (t0 + 2 * TT < t_end) fetch(t0 + 2 * TT);
+      } else {
+#pragma unroll
+        for (int k = 0; k < NL; ++k) {
+          u0[k] = u1[k];
+          z0[k] = z1[k];
+        }
+      }
+      __syncthreads();
+    }
+    if (!CARRY && t_first < t_end) finish(t_first + (t_end - t_first - 1) / TT * TT, k0 ^ 1);
+    return;
   }
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, q = lane % Sh::LN, chl = (warp * Sh::LC + lane / Sh::LN) * C;
