@@ -15,21 +15,16 @@ namespace srwm {
 namespace {
 using namespace scan;
 
-struct Chan4 {
-  float v[4];
-  __device__ __forceinline__ Chan4() { v[0] = v[1] = v[2] = v[3] = 0.f; }
-  __device__ __forceinline__ explicit Chan4(float4 f) { v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w; }
-  __device__ __forceinline__ float4 f4() const { return make_float4(v[0], v[1], v[2], v[3]); }
-};
-
-// w[j][i]: tap j of channel i
+// w[j]: tap j of four channels
 template <int K>
-__device__ __forceinline__ void load_taps(const ConvParams& p, int d, int valid, float (&w)[K][4], float (&b)[4]) {
+__device__ __forceinline__ void load_taps(const ConvParams& p, int d, int valid, Pairs (&w)[K], Pairs& b) {
+  b = four(p.bias ? p.bias + d : nullptr, valid);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    b[i] = i < valid && p.bias ? p.bias[d + i] : 0.f;
+  for (int j = 0; j < K; ++j) {
+    float v[4];
 #pragma unroll
-    for (int j = 0; j < K; ++j) w[j][i] = i < valid ? p.w[(long long)(d + i) * K + j] : 0.f;
+    for (int i = 0; i < 4; ++i) v[i] = i < valid ? p.w[(long long)(d + i) * K + j] : 0.f;
+    w[j] = Pairs(make_float4(v[0], v[1], v[2], v[3]));
   }
 }
 __device__ __forceinline__ bool starts(const ConvParams& p, int n, int t) {
@@ -67,32 +62,27 @@ __global__ void __launch_bounds__(128) conv_fwd_kernel(const ConvParams p) {
   }
 #pragma unroll
   for (int j = 1; j < K; ++j) past[j] = input<T, K, VEC>(p, n, t0 - K + j, d, valid);
-  float w[K][4], b[4];
+  Pairs w[K], b, win[K];       // win: x_{t-K+1} .. x_t
   load_taps<K>(p, d, valid, w, b);
-  Chan4 win[K];       // x_{t-K+1} .. x_t
 #pragma unroll
   for (int j = 1; j < K; ++j) {
     const int t = t0 - K + j;
-    win[j] = Chan4(past[j].get());
+    win[j] = Pairs(past[j].get());
     if (DONE && t >= 0 && starts(p, n, t)) {
 #pragma unroll
-      for (int k = 1; k < j; ++k) win[k] = Chan4();
+      for (int k = 1; k < j; ++k) win[k] = Pairs();
     }
   }
 #pragma unroll
   for (int k = 0; k < TS; ++k) {
     if (t0 + k >= t_end) break;
 #pragma unroll
-    for (int j = 0; j + 1 < K; ++j) win[j] = DONE && cut[k] ? Chan4() : win[j + 1];
-    win[K - 1] = Chan4(row[k].get());
-    Chan4 y;
+    for (int j = 0; j + 1 < K; ++j) win[j] = DONE && cut[k] ? Pairs() : win[j + 1];
+    win[K - 1] = Pairs(row[k].get());
+    Pairs y = b;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float a = b[i];
-#pragma unroll
-      for (int j = 0; j < K; ++j) a = fmaf(w[j][i], win[j].v[i], a);
-      y.v[i] = p.silu ? a * sigmoid(a) : a;
-    }
+    for (int j = 0; j < K; ++j) y = fma4(w[j], win[j], y);
+    if (p.silu) y = y * sigmoid4(y);
     put4<VEC>(py + k * p.y.sl, valid, y.f4());
   }
   if (t_end == p.L && p.sT.p) {
@@ -112,14 +102,10 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
   const int d = ((int)blockIdx.x * 32 + lane) * 4, valid = max(0, min(4, p.D - d));
   const int chunks = (p.L + TS - 1) / TS;
   const long long units = (long long)p.N * chunks;
-  float w[K][4], b[4], dw[K][4], db[4];
+  Pairs w[K], b, dw[K], db;
   load_taps<K>(p, d, valid, w, b);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    db[i] = 0.f;
-#pragma unroll
-    for (int j = 0; j < K; ++j) dw[j][i] = 0.f;
-  }
+  const u64 one = dup2(1.f), minus = dup2(-1.f);
+  const Pairs ones(one, one), minuses(minus, minus);
   for (long long u = (long long)blockIdx.y * 4 + warp; u < units; u += (long long)gridDim.y * 4) {
     if (valid == 0) break;
     const int n = (int)(u / chunks), t0 = (int)(u % chunks) * TS;
@@ -140,17 +126,17 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
     // From the chunk's first step on, K - 1 steps beyond its last: dx[s] (of the state's rows too, in the first chunk) is whole
     // once the step K - 1 behind it is done.  Steps beyond the call's end have no gradient.
     const bool last = t0 + TS > p.L - (K - 1) && p.dsT.p != nullptr;      // some of the inputs are in the state behind the call
-    Chan4 win[K], acc[K];       // acc[j]: of the input at t - K + 1 + j
+    Pairs win[K], acc[K];       // acc[j]: of the input at t - K + 1 + j
     int age = K - 1;            // steps since the episode's start, as far as they matter
 #pragma unroll
     for (int j = 1; j < K; ++j) {
       const int t = t0 - K + j;
-      win[j] = Chan4(past[j].get());
+      win[j] = Pairs(past[j].get());
       if (DONE && t >= 0) {
         const bool cut = starts(p, n, t);
         if (cut) {
 #pragma unroll
-          for (int k = 1; k < j; ++k) win[k] = Chan4();
+          for (int k = 1; k < j; ++k) win[k] = Pairs();
         }
         age = cut ? 0 : min(K - 1, age + 1);
       }
@@ -162,7 +148,7 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
       if (DONE && kept)
         for (int r = max(s + 1, 0); r < p.L; ++r) kept = kept && !starts(p, n, r);
       q.fetch(reinterpret_cast<const T*>(p.dsT.p) + n * p.dsT.sn + (long long)(s - (p.L - (K - 1))) * p.dsT.sl + d, kept ? valid : 0);
-      return Chan4(q.get());
+      return Pairs(q.get());
     };
     if (last) {
 #pragma unroll
@@ -174,13 +160,13 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
       if (t >= p.L + K - 1) break;
 #pragma unroll
       for (int j = 0; j + 1 < K; ++j) acc[j] = acc[j + 1];
-      acc[K - 1] = last ? carried(t) : Chan4();
+      acc[K - 1] = last ? carried(t) : Pairs();
       const bool fresh = DONE && t < p.L && starts(p, n, t);
       if (DONE) age = fresh ? 0 : min(K - 1, age + 1);
 #pragma unroll
-      for (int j = 0; j + 1 < K; ++j) win[j] = DONE && fresh ? Chan4() : win[j + 1];
-      win[K - 1] = Chan4(rx[k % AHEAD].get());
-      const Chan4 go(ry[k % AHEAD].get());
+      for (int j = 0; j + 1 < K; ++j) win[j] = DONE && fresh ? Pairs() : win[j + 1];
+      win[K - 1] = Pairs(rx[k % AHEAD].get());
+      Pairs gp(ry[k % AHEAD].get());
       if (k + AHEAD < ALL) {
         const int v = t + AHEAD < p.L ? valid : 0;
         rx[k % AHEAD].fetch(px, v);
@@ -188,26 +174,22 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
         px += p.x.sl;
         py += p.dy.sl;
       }
+      if (p.silu) {      // silu'(a) = sigmoid (1 + a (1 - sigmoid))
+        Pairs a = b;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float gp = go.v[i];
-        if (p.silu) {
-          float a = b[i];
+        for (int j = 0; j < K; ++j) a = fma4(w[j], win[j], a);
+        const Pairs sg = sigmoid4(a);
+        gp = gp * (sg * fma4(a, fma4(sg, minuses, ones), ones));
+        if (t >= p.L) gp = Pairs();      // (whatever the window holds)
+      }
 #pragma unroll
-          for (int j = 0; j < K; ++j) a = fmaf(w[j][i], win[j].v[i], a);
-          const float sg = sigmoid(a);
-          gp *= sg * fmaf(a, 1.f - sg, 1.f);
-          if (t >= p.L) gp = 0.f;      // (whatever the window holds)
-        }
+      for (int j = 0; j < K; ++j)
+        if (!DONE || K - 1 - j <= age) acc[j] = fma4(w[j], gp, acc[j]);
+      if (k < TS) {
+        db = db + gp;
 #pragma unroll
         for (int j = 0; j < K; ++j)
-          if (!DONE || K - 1 - j <= age) acc[j].v[i] = fmaf(w[j][i], gp, acc[j].v[i]);
-        if (k < TS) {
-          db[i] += gp;
-#pragma unroll
-          for (int j = 0; j < K; ++j)
-            if (!DONE || K - 1 - j <= age) dw[j][i] = fmaf(gp, win[j].v[i], dw[j][i]);
-        }
+          if (!DONE || K - 1 - j <= age) dw[j] = fma4(gp, win[j], dw[j]);
       }
       if (k >= K - 1) {
         put4<VEC>(ox, t - (K - 1) < p.L ? valid : 0, acc[0].f4());
@@ -220,9 +202,8 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
   float* out = p.part + (long long)blockIdx.y * p.D * (K + 1);
 #pragma unroll
   for (int j = 0; j <= K; ++j) {
-    const float* v = j < K ? dw[j < K ? j : 0] : db;
     __syncthreads();
-    red[warp][lane] = make_float4(v[0], v[1], v[2], v[3]);
+    red[warp][lane] = (j < K ? dw[j < K ? j : 0] : db).f4();
     __syncthreads();
     if (warp == 0) {
       float4 s = red[0][lane];

@@ -19,10 +19,10 @@ namespace srwm {
 namespace {
 using namespace scan;
 
-// A row's threads: a warp (eight rows a block) or the whole block
-template <bool BLOCK>
+// A row's threads: a warp (some rows a block) or the whole block
+template <bool BLOCK, int THREADS = 256>
 struct Team {
-  static constexpr int SIZE = BLOCK ? 256 : 32, ROWS = 256 / SIZE;
+  static constexpr int SIZE = BLOCK ? 256 : 32, ROWS = THREADS / SIZE;
   static __device__ __forceinline__ float sum(float v, float* red) {
     v = allreduce_warp(v);
     if constexpr (BLOCK) {
@@ -67,9 +67,9 @@ inline bool quads_ok(const void* p, long long row, int D, int es) { return (uint
 
 // NV: pieces of four columns of a thread
 template <typename T, bool VEC, bool BLOCK, int NV, bool FP8>
-__global__ void __launch_bounds__(256) rms_fwd_kernel(const RmsParams p) {
+__global__ void __launch_bounds__(BLOCK ? 256 : 128) rms_fwd_kernel(const RmsParams p) {
   chained();
-  using G = Team<BLOCK>;
+  using G = Team<BLOCK, BLOCK ? 256 : 128>;
   __shared__ float red[8];
   const int lane = threadIdx.x % G::SIZE, sub = threadIdx.x / G::SIZE;
   const float inv_d = 1.f / (float)p.D;
@@ -250,10 +250,11 @@ cudaError_t rms_forward(const RmsParams& p, cudaStream_t s) {
     using T = decltype(t);
     constexpr bool V = decltype(v)::value, B = decltype(block)::value;
     constexpr int NV = decltype(nv)::value;
-    const long long blocks = (p.rows + Team<B>::ROWS - 1) / Team<B>::ROWS, most = 16ll * common_sms();
+    constexpr int THREADS = B ? 256 : 128, ROWS = Team<B, THREADS>::ROWS;
+    const long long blocks = (p.rows + ROWS - 1) / ROWS, most = 32ll * common_sms();
     const dim3 grid((unsigned)(blocks < most ? blocks : most));
-    return p.fp8 ? launch_behind(rms_fwd_kernel<T, V, B, NV, true>, p, grid, 256, 0, s)
-                 : launch_behind(rms_fwd_kernel<T, V, B, NV, false>, p, grid, 256, 0, s);
+    return p.fp8 ? launch_behind(rms_fwd_kernel<T, V, B, NV, true>, p, grid, THREADS, 0, s)
+                 : launch_behind(rms_fwd_kernel<T, V, B, NV, false>, p, grid, THREADS, 0, s);
   });
 }
 cudaError_t rms_backward(const RmsParams& p, cudaStream_t s) {

@@ -247,14 +247,15 @@ __global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 ? 1 : 2) s
 }
 
 // A few steps, states in registers, everything else straight from memory: what an actor or a server does for each token.  Bound by the state's
-// bytes, and by its launch where these are few.  NB: sequences of a thread, whose loads are all on their way before the first is used; more
-// than one where there are enough of them (256 sequences x 2048 channels, S 16, bf16: 34 us with one, see the rule).
+// bytes, and by its launch where these are few.  NB: sequences of a thread.  With four, what belongs to a channel and sequence (softplus,
+// gate) is formed by one of the channel's lanes each and passed around; with one, by all of them (256 sequences x 2048 channels, S 16,
+// bf16: 33 us with one, 25 with four and no passing around).
 template <typename T, int S, bool VEC, int NB>
 __global__ void __launch_bounds__(Shape<S, 1, SCAN_TILE>::WALK) scan_step_kernel(const ScanParams p) {
   using Sh = Shape<S, 1, SCAN_TILE>;
-  constexpr int NP = Sh::NP;
+  constexpr int NP = Sh::NP, LN = Sh::LN, OWN = NB > LN ? NB / LN : 1;      // OWN: sequences whose values a lane forms
   chained();
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, q = lane % Sh::LN, chl = warp * Sh::LC + lane / Sh::LN;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, q = lane % LN, chl = warp * Sh::LC + lane / LN;
   const Place<Sh::CH> at(p, blockIdx.x);       // (its n: of the first of NB sequences, counted in such groups)
   const int n0 = at.n * NB;
   const bool mine = chl < at.left;
@@ -269,17 +270,21 @@ __global__ void __launch_bounds__(Shape<S, 1, SCAN_TILE>::WALK) scan_step_kernel
   load_states<Sh>(p.A + (long long)d * S, q, A2);
   const float bias = p.bias ? p.bias[d] : 0.f, skip = p.skip ? p.skip[d] : 0.f;
   for (int t = 0; t < p.L; ++t) {
-    float u[NB], x[NB], z[NB];
+    float u[OWN], x[OWN], z[OWN];
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      const long long n = min(n0 + (NB == 1 ? 0 : (q + o * LN) % NB), p.N - 1);
+      u[o] = to_float(reinterpret_cast<const T*>(p.u.p)[n * p.u.sn + t * p.u.sl + d]);
+      x[o] = to_float(reinterpret_cast<const T*>(p.delta.p)[n * p.delta.sn + t * p.delta.sl + d]) + bias;
+      z[o] = p.z.p ? to_float(reinterpret_cast<const T*>(p.z.p)[n * p.z.sn + t * p.z.sl + d]) : 0.f;
+    }
     bool fresh[NB];
     u64 b2[NB][NP], c2[NB][NP];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int n = min(n0 + b, p.N - 1);
-      u[b] = to_float(reinterpret_cast<const T*>(p.u.p)[n * p.u.sn + t * p.u.sl + d]);
-      x[b] = to_float(reinterpret_cast<const T*>(p.delta.p)[n * p.delta.sn + t * p.delta.sl + d]);
-      z[b] = p.z.p ? to_float(reinterpret_cast<const T*>(p.z.p)[n * p.z.sn + t * p.z.sl + d]) : 0.f;
+      const long long n = min(n0 + b, p.N - 1);
       fresh[b] = p.done && p.done[n * p.done_n + t * p.done_l] != 0;
-      auto row = [&](const ScanRows& w, u64 (&v)[NP]) {
+      auto row = [&](const ScanRows& w, u64* v) {
         const T* r = reinterpret_cast<const T*>(w.p) + n * w.sn + at.g * w.sg + t * w.sl;
 #pragma unroll
         for (int i = 0; i < Sh::ST / 4; ++i) {
@@ -293,24 +298,49 @@ __global__ void __launch_bounds__(Shape<S, 1, SCAN_TILE>::WALK) scan_step_kernel
       row(p.B, b2[b]);
       row(p.C, c2[b]);
     }
+    float dl[OWN], du[OWN], y[NB];
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      dl[o] = p.softplus ? softplus(x[o]) : x[o];
+      du[o] = dl[o] * u[o];
+      dl[o] *= LOG2E;
+    }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const float dl = p.softplus ? softplus(x[b] + bias) : x[b] + bias;
-      const u64 d2 = dup2(dl * LOG2E), x2 = dup2(dl * u[b]);
+      const float db = NB == 1 ? dl[0] : __shfl_sync(0xffffffffu, dl[b / LN], b % LN, LN);
+      const float xb = NB == 1 ? du[0] : __shfl_sync(0xffffffffu, du[b / LN], b % LN, LN);
       u64 acc = 0ull;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        u64 a = exp2_pair(mul2(d2, A2[i]));
+        u64 a = exp2_pair(mul2(dup2(db), A2[i]));
         if (fresh[b]) a = h[b][i] = 0ull;
-        h[b][i] = fma2<true>(a, h[b][i], mul2(x2, b2[b][i]));
-        acc = fma2<true>(h[b][i], c2[b][i], acc);
+        h[b][i] = fma2<true>(a, h[b][i], mul2(dup2(xb), b2[b][i]));
+        acc = i == 0 ? mul2(h[b][i], c2[b][i]) : fma2<true>(h[b][i], c2[b][i], acc);
       }
-      float y = hsum2(acc);
+      y[b] = hsum2(acc);
+    }
+    // the sums over the lanes; with four sequences lane q ends with those of its own
+    constexpr int W = NB < LN ? NB : LN;
 #pragma unroll
-      for (int w = 1; w < Sh::LN; w *= 2) y += __shfl_xor_sync(0xffffffffu, y, w);
-      y = fmaf(skip, u[b], y);
-      if (p.z.p) y *= z[b] * sigmoid(z[b]);
-      if (mine && q == 0 && n0 + b < p.N) narrow(y, reinterpret_cast<T*>(p.y.p) + (n0 + b) * p.y.sn + t * p.y.sl + d);
+    for (int w = W; w < LN; w *= 2) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) y[b] += __shfl_xor_sync(0xffffffffu, y[b], w);
+    }
+#pragma unroll
+    for (int w = 1; w < W; w *= 2) {
+      const bool up = q & w;
+#pragma unroll
+      for (int b = 0; b < NB; b += 2 * w) {
+        const float keep = up ? y[b + w] : y[b], send = up ? y[b] : y[b + w];
+        y[b] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+      }
+    }
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      const int b = q + o * LN;
+      float r = fmaf(skip, u[o], y[o * LN < NB ? o * LN : 0]);
+      if (p.z.p) r *= z[o] * sigmoid(z[o]);
+      if (mine && b < NB && n0 + b < p.N) narrow(r, reinterpret_cast<T*>(p.y.p) + (long long)(n0 + b) * p.y.sn + t * p.y.sl + d);
     }
   }
   if (!mine || !p.hT) return;
@@ -338,7 +368,7 @@ cudaError_t sequences(const ScanParams& p, cudaStream_t s) {
 template <typename T, int S, bool VEC>
 cudaError_t launch(const ScanParams& p, cudaStream_t s) {
   if (p.L <= SCAN_STEPS_DIRECT && !p.ckpt) {
-    constexpr int NB = S <= 16 ? 4 : 2;
+    constexpr int NB = 4;
     const long long grid = blocks_of(p, Shape<S, 1, SCAN_TILE>::CH);
     if (grid < 32 * common_sms()) return launch_behind(scan_step_kernel<T, S, VEC, 1>, p, dim3((unsigned)grid), Shape<S, 1, SCAN_TILE>::WALK, 0, s);
     return launch_behind(scan_step_kernel<T, S, VEC, NB>, p, dim3((unsigned)(grid / p.N * ((p.N + NB - 1) / NB))), Shape<S, 1, SCAN_TILE>::WALK, 0, s);
