@@ -16,6 +16,9 @@ but the per-call work around the operator -- input softmax, four ``W.repeat(bsz,
 (``layer_ops.srwm_layer`` / ``layer_ops.delta_layer``).
 ``SRlayer.unroll`` additionally runs the learner's one-step-at-a-time loop with episode
 resets (reinforcement_learning/torchbeast_procgen/model.py:1180-1197) as ONE call.
+
+``SSMlayer`` is a selective state-space layer with the same time-major conventions, to stack or compare with the fast-weight
+layers (no reference layer corresponds): root-mean-square norm, projection, ``causal_conv``, ``selective_scan``, projection, residual.
 """
 from __future__ import annotations
 
@@ -26,6 +29,8 @@ import torch.nn as nn
 
 from . import _lib as L
 from .layer_ops import delta_layer, srwm_layer
+from .norm_ops import rms_norm
+from .scan_ops import causal_conv, selective_scan
 
 
 # The modules' linear maps and layer norms run on this library's kernels (fp32 in and out; the products
@@ -281,3 +286,66 @@ class FastFFlayerRL(FastFFlayer):
         out = delta_layer(self._rows(x), state, norm_eps=self.norm_eps)
         return _project(self.out_linear, self.drop, _merge(out), x), state.clone()
 
+
+
+class SSMlayer(nn.Module):
+    """Selective state-space layer: ``out = s + out_linear(selective_scan(...))`` on the normalised stream s.
+
+        out = layer(h)                                  h [L, B, in_dim], time-major as the other layers
+        out, state = layer(h, state, done=done, get_state=True)
+        out = layer(h, residual=stream)                 s = h + stream, added in the norm's kernel
+
+    ``state``: (the convolution's last inputs [B, taps - 1, inner], the scan's state [B, inner, state_dim] float32), from
+    ``init_state`` or the call before; gradients flow through it (detach it where they should not).  ``done [L, B]``: before
+    step t the state of the samples with ``done[t]`` goes back to zero.  ``inplace_state`` (without gradients, an actor's
+    step): the given state is advanced in place, also in a captured graph.
+    """
+
+    def __init__(self, in_dim, dropout=0.0, state_dim=16, expand=2, taps=4, step_rank=None, norm_eps=1e-6):
+        super().__init__()
+        inner = expand * in_dim
+        rank = step_rank if step_rank is not None else max(4, in_dim // 64 * 4)
+        self.in_dim, self.inner, self.state_dim, self.taps, self.rank, self.norm_eps = in_dim, inner, state_dim, taps, rank, norm_eps
+        self.norm_weight = nn.Parameter(torch.ones(in_dim))
+        self.in_linear = nn.Linear(in_dim, 2 * inner, bias=False)             # the convolution's rows and the gate's
+        self.conv_weight = nn.Parameter(torch.empty(inner, taps))
+        self.conv_bias = nn.Parameter(torch.zeros(inner))
+        self.x_linear = nn.Linear(inner, rank + 2 * state_dim, bias=False)    # step size (low rank), B, C
+        self.step_linear = nn.Linear(rank, inner, bias=False)
+        self.step_bias = nn.Parameter(torch.empty(inner))
+        self.A_log = nn.Parameter(torch.empty(inner, state_dim))
+        self.D = nn.Parameter(torch.ones(inner))
+        self.out_linear = nn.Linear(inner, in_dim, bias=False)
+        self.drop = nn.Dropout(dropout)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        """Decays from 1 to state_dim, step sizes between 0.001 and 0.1."""
+        nn.init.uniform_(self.conv_weight, -self.taps ** -0.5, self.taps ** -0.5)
+        with torch.no_grad():
+            step = torch.exp(torch.empty_like(self.step_bias).uniform_(math.log(1e-3), math.log(1e-1)))
+            self.step_bias.copy_(step + torch.log(-torch.expm1(-step)))
+            self.A_log.copy_(torch.arange(1, self.state_dim + 1, device=step.device).log().expand_as(self.A_log))
+
+    def init_state(self, bsz):
+        like = self.in_linear.weight
+        return (like.new_zeros(bsz, self.taps - 1, self.inner),
+                torch.zeros(bsz, self.inner, self.state_dim, device=like.device))
+
+    def forward(self, h, state=None, done=None, get_state=False, residual=None, inplace_state=False):
+        x = rms_norm(h, self.norm_weight.float(), residual=residual, eps=self.norm_eps)
+        if residual is not None:
+            x, h = x
+        conv_state, scan_state = (None, None) if state is None else state
+        done = None if done is None else done.t()
+        xz = _linear(self.in_linear, x).transpose(0, 1)                   # [B, L, .] views from here on
+        x, z = xz[..., :self.inner], xz[..., self.inner:]
+        x, conv_state = causal_conv(x, self.conv_weight.float(), self.conv_bias.float(), conv_state, done, True, inplace_state)
+        rows = _linear(self.x_linear, x.transpose(0, 1))
+        step = _linear(self.step_linear, rows[..., :self.rank].contiguous()).transpose(0, 1)
+        rows = rows.transpose(0, 1)
+        B, C = rows[..., self.rank:self.rank + self.state_dim], rows[..., self.rank + self.state_dim:]
+        y, scan_state = selective_scan(x, step, -torch.exp(self.A_log.float()), B, C, self.D.float(), z, self.step_bias.float(),
+                                       scan_state, done, True, inplace_state)
+        out = _project(self.out_linear, self.drop, y.transpose(0, 1), h)
+        return (out, (conv_state, scan_state)) if get_state else out
