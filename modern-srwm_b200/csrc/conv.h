@@ -7,10 +7,11 @@
 
 namespace srwm {
 
-constexpr int CONV_CHUNK = 16;     // steps of a thread at most
+constexpr int CONV_CHUNK = 16;     // steps of a thread at least (a shorter call is one chunk)
 
 struct ConvParams {
   int N, L, D, K;
+  int chunk;                       // steps of a thread (set by the launch)
   int bf16, silu, vec;             // vec: all rows' pieces of four channels are aligned to their size
   ScanRows x, y, s0, sT;           // [N, L, D]; the states [N, K-1, D], NULL: zeros / not wanted
   const float *w, *bias;           // [D, K], [D] or NULL
