@@ -376,7 +376,7 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
     // Four steps at a time, the last first.  The second four have the first four walked on the way to them (without what they leave), so that a
     // and a h of no more than four stay in registers.
     auto tile = [&](auto whole) __attribute__((always_inline)) {
-      constexpr bool WHOLE = decltype(whole)::value;
+      constexpr bool WHOLE = decltype(whole)::value;      // eight steps of one episode, all channels there
 #pragma unroll 1
       for (int s0 = SUB; s0 >= 0; s0 -= SUB) {
         if (!WHOLE && s0 >= steps) continue;
@@ -450,7 +450,8 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
                 ah[k][c][i] = mul2(a[k][c][i], h[c][i]);
                 h[c][i] = add2(ah[k][c][i], in);
                 acc = i == 0 ? mul2(h[c][i], c2[i]) : fma2<true>(h[c][i], c2[i], acc);
-                sum[i] = c == 0 ? mul2(h[c][i], g2) : fma2<true>(h[c][i], g2, sum[i]);
+                const u64 share = WHOLE || c < mine ? h[c][i] : 0ull;      // (no channel: B may be infinite, and 0 B not 0)
+                sum[i] = c == 0 ? mul2(share, g2) : fma2<true>(share, g2, sum[i]);
               }
               y[c] = hsum2(acc);
             }
@@ -485,7 +486,8 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
                 gb = i == 0 ? mul2(g, b2[i]) : fma2<true>(g, b2[i], gb);
                 sa = i == 0 ? mul2(gah, A2[c][i]) : fma2<true>(gah, A2[c][i], sa);
                 dA[c][i] = fma2<true>(gah, d2, dA[c][i]);
-                sum[i] = c == 0 ? mul2(g, x2) : fma2<true>(g, x2, sum[i]);
+                const u64 share = WHOLE || c < mine ? g : 0ull;
+                sum[i] = c == 0 ? mul2(share, x2) : fma2<true>(share, x2, sum[i]);
                 gc[c][i] = fresh ? 0ull : mul2(a[k][c][i], g);
               }
               gbv[c] = hsum2(gb);
@@ -503,7 +505,7 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
         }
       }
     };
-    if (steps == TT && now == 0u) tile(std::true_type());
+    if (steps == TT && now == 0u && at.left >= CH) tile(std::true_type());
     else tile(std::false_type());
     __syncthreads();
   }

@@ -192,6 +192,49 @@ def test_scan_masked_and_infinite_values_stay_where_they_belong():
     assert torch.equal(y[:, :, keep], sb.selective_scan(**{**x, "delta_bias": None}, done=done)[0][:, :, keep])
 
 
+@pytest.mark.parametrize("D", [1, 33])
+def test_scan_infinite_b_and_c(D):
+    """An infinite B or C reaches the gradients that it has a part in, and the channels that a block has room for beyond D none."""
+    for name in ("B", "C"):
+        x, _, gy, gs = _inputs(1, 20, D, 16, 1, torch.float32, seed=12)
+        x[name][0, 13, 5] = float("inf")
+        ref = {k: v.detach().double().requires_grad_() for k, v in x.items()}
+        want = torch.autograd.grad(list(orc.scan(**ref)), [ref["B"], ref["C"]], [gy.double(), gs.double()])
+        args = {k: v.detach().requires_grad_() for k, v in x.items()}
+        got = torch.autograd.grad(list(sb.selective_scan(**args)), [args["B"], args["C"]], [gy, gs])
+        for a, b in zip(got, want):
+            assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.isposinf(), b.isposinf()) and torch.equal(a.isneginf(), b.isneginf())
+            fine = torch.isfinite(b)
+            _near(torch.where(fine, a, torch.zeros_like(a)), torch.where(fine, b, torch.zeros_like(b)), GRAD, name)
+
+
+def test_rows_beyond_32_bit_offsets():
+    """Sequences more than 2^31 elements apart, and a tensor of more than 2^31 values."""
+    far = (1 << 31) + 64
+    buf = torch.zeros(far + 40 * 96, device="cuda", dtype=torch.bfloat16)
+    view = lambda w, at=0: buf.as_strided((2, 40, w), (far, 96, 1), at)  # noqa: E731
+    x, _, gy, _ = _inputs(2, 40, 32, 16, 1, torch.bfloat16, seed=13)
+    for k, at in (("u", 0), ("z", 32), ("C", 64)):
+        view(x[k].shape[-1], at).copy_(x[k])
+    near, far_ = [{k: v.detach().clone().requires_grad_() for k, v in x.items()} for _ in range(2)]
+    for k, at in (("u", 0), ("z", 32), ("C", 64)):
+        far_[k] = view(x[k].shape[-1], at).detach().requires_grad_()
+    a, b = sb.selective_scan(**near), sb.selective_scan(**far_)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for g, h in zip(torch.autograd.grad(a[0], list(near.values()), gy), torch.autograd.grad(b[0], list(far_.values()), gy)):
+        assert torch.equal(g, h)
+    w = torch.randn(32, 4, device="cuda")
+    near_u = x["u"].clone().requires_grad_()
+    c, d = sb.causal_conv(near_u, w), sb.causal_conv(far_["u"], w)
+    assert torch.equal(c[0], d[0]) and torch.equal(torch.autograd.grad(c[0].sum(), near_u)[0], torch.autograd.grad(d[0].sum(), far_["u"])[0])
+    n = torch.ones(32, device="cuda")
+    assert torch.equal(sb.rms_norm(x["u"][:, 3], n), sb.rms_norm(view(32)[:, 3], n))
+    want = float(buf[:4096].double().square().sum() + buf[-4096:].double().square().sum()) ** 0.5      # (zeros between)
+    assert abs(float(sb.grad_norm([buf])) / want - 1) < 1e-6
+    sb.grad_ops.clip_tensors_([buf], want / 2)
+    assert abs(float(sb.grad_norm([buf])) / (want / 2) - 1) < 2e-3
+
+
 def test_scan_small_steps_keep_their_precision():
     """Steps of 1e-3 and slow decays: 1000 steps of memory; the state's relative error is a random walk of half-steps of the decay,
     2^-24 sqrt(1000) = 2e-6, and at most the sum of the exponentials' bias: 1e-5 asked."""
