@@ -3,7 +3,9 @@
 // with the K - 1 inputs before the call carried as a state, and none read across an episode's start.
 //
 // Bound by HBM: one read and one write of [N, L, D].  A thread takes four channels and a chunk of steps in time order, its window in
-// registers, the next steps' rows on their way; the K - 1 steps in front of its own come from L2.
+// registers, the next steps' rows on their way; the K - 1 steps in front of its own come from L2.  8 x 2048 x 2048, K 4, bf16: forward 32 us
+// (21 at the copy bandwidth), backward 57 (31).  Chunks as long as fill the GPU once, and steps inside a chunk without conditions, took
+// them there from 39 and 75 with chunks of 16: the backward's instructions bind, a hundred for four channels and a step.
 #include <type_traits>
 
 #include "chain.h"

@@ -5,8 +5,13 @@
 //   du_t = D dy'_t + Delta_t (g_t . B_t)        dDelta_t = u_t (g_t . B_t) + sum_s A a_t h_{t-1} g_t
 // A CTA takes its 64 (32) channels from the last step to the first.  The states in front of each eighth step are the forward's; within
 // eight steps they are formed again, four at a time, a_t and a_t h_{t-1} staying in registers until the way back has used them.  Thirteen fp32
-// operations per state and step bind.  Sums over states go through a channel's lanes, sums over channels (dB, dC) through the
-// warp's other lanes and shared memory, and are added up over the CTAs by a second launch, in a fixed order.
+// operations per state and step are its floor.  Sums over states go through shared memory, a row a lane; sums over channels (dB, dC) through
+// the warp's lanes and shared memory, and are added up over the CTAs by a second launch, in a fixed order.
+//
+// 8 sequences x 2048 steps x 2048 channels, S 16, bf16: 738 us (1580 with every warp loading, walking and writing in turn and one channel
+// a thread).  Four walking and four loading warps a CTA, two CTAs a multiprocessor by registers: issue is busy 53 % of the time, the
+// fp32 pipe 43, shared memory 60; a scheduler has two walking warps, and each waits for its own chain.  Sums over lanes by shuffles, with
+// selects, took 780; states of eight steps in registers spill at 168 a thread (2250).
 #include <type_traits>
 
 #include "device.h"
@@ -104,7 +109,7 @@ struct BwdSmem {
   float4 sums[2][Sh::PIECES];    // of dy' u and of the gradient of delta, a slot for each loading thread's piece
 };
 
-// Registers: the walking threads' share and the loading threads', which together are at most what the CTA is launched with (128 a thread, two
+// Registers: the walking threads' share and the loading threads' (88 for these spill: 1150 us against 970 forward and backward), which together are at most what the CTA is launched with (128 a thread, two
 // CTAs a multiprocessor; S 64: 168 and one): a share beyond that would be waited for without end.
 template <int S>
 struct BwdRegs {

@@ -17,10 +17,14 @@ struct FwdSmem {
 };
 
 // CARRY: only what a piece of the time axis makes of the state (its end from zero, and the product of its decays), for the
-// pieces behind it; one CTA per 32 channels and piece.  Four warps load and prepare a tile, and write
-// the one before it, while the others walk the tile between: one barrier a tile.
+// pieces behind it; one CTA per 32 or 64 channels and piece.
+//
+// Four warps load and prepare a tile, and write the one before it, while the others walk the tile between: one barrier a tile.  8 sequences x
+// 2048 steps x 2048 channels, S 16, bf16: 229 us, of which the exponentials alone are 119 (their pipe is busy 60 % of the time, issue 52 %);
+// with the loading in the same warps 264, with one channel a thread 288, without the exponentials formed ahead of the chain 341.
+// 256 CTAs are two on some multiprocessors and one on others, 14 % of it.
 template <typename T, int S, bool VEC, int C, bool CARRY>
-__global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 ? 1 : 2) scan_fwd_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 && C == 2 ? 1 : 2) scan_fwd_kernel(const ScanParams p) {
   using Sh = Shape<S, C, SCAN_TILE>;
   constexpr int TT = SCAN_TILE, CH = Sh::CH, NP = Sh::NP, NL = Sh::NL, NQ = Sh::NQ, BUFS = CARRY ? 1 : 2;
   extern __shared__ __align__(16) unsigned char raw_smem[];
@@ -170,7 +174,7 @@ __global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 ? 1 : 2) s
     // ahead of the chain through it, so that the exponentials' pipe does not wait for it either.
     auto walk = [&](auto whole) {
       constexpr bool WHOLE = decltype(whole)::value;
-      constexpr int PU = 16 / (C * Sh::ST) < 1 ? 1 : 16 / (C * Sh::ST);
+      constexpr int PU = Sh::ST == 8 ? 1 : 4 / C;      // (eight states a thread: 438 us with two, 411 with one; S 64, 8 x 2048 x 1024, bf16)
       u64 a[2][PU][C][NP], in[2][PU][C][NP], c2[2][PU][NP];
       auto ahead = [&](int t1, int b) __attribute__((always_inline)) {      // steps t1 .. t1 + PU - 1
 #pragma unroll
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 ? 1 : 2) s
 // A few steps, states in registers, everything else straight from memory: what an actor or a server does for each token.  Bound by the state's
 // bytes, and by its launch where these are few.  NB: sequences of a thread.  With four, what belongs to a channel and sequence (softplus,
 // gate) is formed by one of the channel's lanes each and passed around; with one, by all of them (256 sequences x 2048 channels, S 16,
-// bf16: 33 us with one, 25 with four and no passing around).
+// bf16: 17.5 us; 33 with one, 25 with four and no passing around).
 template <typename T, int S, bool VEC, int NB>
 __global__ void __launch_bounds__(Shape<S, 1, SCAN_TILE>::WALK) scan_step_kernel(const ScanParams p) {
   using Sh = Shape<S, 1, SCAN_TILE>;
@@ -368,12 +372,13 @@ cudaError_t sequences(const ScanParams& p, cudaStream_t s) {
 template <typename T, int S, bool VEC>
 cudaError_t launch(const ScanParams& p, cudaStream_t s) {
   if (p.L <= SCAN_STEPS_DIRECT && !p.ckpt) {
-    constexpr int NB = 4;
+    constexpr int NB = 4;      // (48 sequences x 512 channels leave most of the GPU idle either way: the launch is what counts there)
     const long long grid = blocks_of(p, Shape<S, 1, SCAN_TILE>::CH);
     if (grid < 32 * common_sms()) return launch_behind(scan_step_kernel<T, S, VEC, 1>, p, dim3((unsigned)grid), Shape<S, 1, SCAN_TILE>::WALK, 0, s);
     return launch_behind(scan_step_kernel<T, S, VEC, NB>, p, dim3((unsigned)(grid / p.N * ((p.N + NB - 1) / NB))), Shape<S, 1, SCAN_TILE>::WALK, 0, s);
   }
-  // two channels a thread where these CTAs still fill the multiprocessors
+  // two channels a thread where these CTAs still fill the multiprocessors: 8 x 1024 x 2048, S 32, 184 us against 208 (S 64: 346 against
+  // 373); 8 x 2048 x 1024, S 64 (128 CTAs), 376 with one against 411
   if constexpr (S > 8)
     if (blocks_of(p, Shape<S, 2, SCAN_TILE>::CH) * p.nseg >= 1 * common_sms()) return sequences<T, S, VEC, 2>(p, s);
   return sequences<T, S, VEC, 1>(p, s);

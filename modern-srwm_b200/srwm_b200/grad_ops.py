@@ -25,20 +25,16 @@ def grad_norm(tensors):
     return _checked(tensors, -1.0) if r is NotImplemented else r
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
-    if isinstance(parameters, torch.Tensor):
-        parameters = (parameters,)
-    parameters = list(parameters)
-    if not error_if_nonfinite and 0.0 <= float(max_norm):
-        r = L.host().grads_norm(parameters, float(max_norm), True)
+    if type(parameters) is not list:
+        parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    if not error_if_nonfinite and max_norm >= 0.0:
+        r = L.host().grads_norm(parameters, max_norm, True)
         if r is not NotImplemented:
             return r
-    grads = [p.grad for p in parameters if p.grad is not None]
-    return clip_tensors_(grads, max_norm, error_if_nonfinite)
+    return clip_tensors_([p.grad for p in parameters if p.grad is not None], max_norm, error_if_nonfinite)
 
 
-@torch.no_grad()
 def clip_tensors_(grads, max_norm, error_if_nonfinite=False):
     """``clip_grad_norm_`` on the gradients themselves."""
     max_norm = float(max_norm)
@@ -46,12 +42,14 @@ def clip_tensors_(grads, max_norm, error_if_nonfinite=False):
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if not grads:
         return torch.zeros(())
+    grads = list(grads)
     if error_if_nonfinite and not torch.isfinite(norm := grad_norm(grads)):
         raise RuntimeError(f"the norm of the gradients is not finite ({float(norm)}); they have not been scaled")
     r = L.host().grads_norm(grads, max_norm, False)
     return _checked(grads, max_norm) if r is NotImplemented else r
 
 
+@torch.no_grad()
 def _checked(tensors, max_norm):
     device = tensors[0].device
     for t in tensors:
