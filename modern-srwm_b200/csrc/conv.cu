@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(1024) conv_sums_kernel(const ConvSums a) {
   else if (a.dbias) a.dbias[d] = t;
 }
 
-constexpr int CONV_FWD_THREADS = 640;      // of a multiprocessor at once (bf16, 96 registers a thread; 512 with fp32 rows)
+constexpr int CONV_FWD_THREADS = 768;      // of a multiprocessor at once (bf16: six blocks at 80 registers a thread; 640 and 1280 take as long)
 
 // Steps of a chunk, so that the N sequences' chunks are as many as are taken at once; 16 at least (each reads K - 1 steps in front of its own)
 int chunk_of(const ConvParams& p, long long at_once) {
