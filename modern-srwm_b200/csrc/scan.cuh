@@ -6,7 +6,7 @@
 // exponential and four fp32 operations: with 16 exponentials and 128 fp32 operations a cycle and multiprocessor, the exponentials
 // bind (the streams are 8 bytes a channel and step in bf16, read and written in less time than 16 states' exponentials take).  So a thread holds some
 // states of one or two channels in registers and walks the time axis; LN neighbouring lanes share a channel.  What belongs to a channel and
-// step (softplus, the gate) is formed once per tile of 16 steps x 32 or 64 channels, by the thread that loads it.
+// step (softplus, the gate) is formed once, by the thread that loads it into a tile of 16 (8) steps x 32, 64 or 128 channels.
 #pragma once
 #include <type_traits>
 

@@ -25,7 +25,7 @@ struct ScanParams {
   const uint8_t* done;
   long long done_n, done_l;
   float* ckpt;                  // [N][ceil(L / SCAN_CKPT)][D][S], the state in front of each eighth step
-  float* carry;                 // nseg > 1: see scan_scratch_floats
+  float* carry;                 // nseg > 1: each piece's end from zero and the product of its decays, [N][D][S] each (forward: the first state in front)
   // backward
   ScanRows dy, du, ddelta, dz, dB, dC;
   const float* dhT;
@@ -34,7 +34,7 @@ struct ScanParams {
 };
 
 __host__ __device__ constexpr int scan_bwd_channels(int S) { return S == 8 ? 128 : S == 16 ? 64 : 32; }      // of a CTA of the backward
-constexpr int SCAN_FWD_CHANNELS = 64;                     // of a CTA of the forward (32 where these would not fill the GPU)
+constexpr int SCAN_FWD_CHANNELS = 64;                     // of a CTA of the forward (32 where these would not fill the GPU; S 8: 64)
 int scan_segments(const ScanParams& p, int channels, int sms);      // pieces that a call's time axis is cut into
 long long scan_fwd_scratch(const ScanParams& p);           // floats
 long long scan_bwd_scratch(ScanParams& p, float* base);    // floats; base not NULL: sets the pointers into it

@@ -340,6 +340,8 @@ class SSMlayer(nn.Module):
         done = None if done is None else done.t()
         xz = _linear(self.in_linear, x).transpose(0, 1)                   # [B, L, .] views from here on
         x, z = xz[..., :self.inner], xz[..., self.inner:]
+        if conv_state is not None and not inplace_state:
+            conv_state = conv_state.to(x.dtype)       # (under autocast the projections' type is not the weights')
         x, conv_state = causal_conv(x, self.conv_weight.float(), self.conv_bias.float(), conv_state, done, True, inplace_state)
         rows = _linear(self.x_linear, x.transpose(0, 1))
         step = _linear(self.step_linear, rows[..., :self.rank].contiguous()).transpose(0, 1)

@@ -82,6 +82,35 @@ def test_scan_resets_groups_and_pieces_of_time(N, L, D, S, G, dtype):
     _scan_case(N, L, D, S, G, dtype, seed=4, done=True, time_major=True, softplus=False)
 
 
+@pytest.mark.parametrize("N,L,D,S,G,dtype", [(40, 35, 250, 16, 1, torch.float32), (40, 35, 256, 16, 2, torch.bfloat16), (40, 21, 256, 32, 1, torch.float32),
+                                             (40, 37, 250, 32, 2, torch.bfloat16), (38, 20, 256, 64, 1, torch.float32), (40, 19, 250, 64, 2, torch.bfloat16),
+                                             (40, 35, 300, 8, 1, torch.float32), (2, 1200, 512, 16, 1, torch.float32), (37, 300, 64, 64, 1, torch.float32),
+                                             (2, 1100, 576, 32, 1, torch.bfloat16)])
+def test_scan_grids_that_fill_the_gpu(N, L, D, S, G, dtype):
+    """Two channels a thread; the last three cut into pieces of the time axis as well (no sum has more than 300 terms in a row then either:
+    a piece's steps, the pieces and sequences, the channels of a block, the blocks)."""
+    _scan_case(N, L, D, S, G, dtype, done=True)
+    _scan_case(N, L, D, S, G, dtype, seed=2, gate=False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("S", [8, 16, 32, 64])
+@pytest.mark.parametrize("N,L,D,G", [(303, 1, 1000, 1), (301, 3, 1028, 2)])
+def test_tokens_of_many_sequences(N, L, D, G, S, dtype):
+    """Four sequences a thread, the last group not whole."""
+    x, done, _, _ = _inputs(N, L, D, S, G, dtype, seed=21, done=True)
+    with torch.no_grad():
+        yr, hr = orc.scan(**{k: v.double() for k, v in x.items()}, done=done)
+        st = x["state"].clone()
+        y, h = sb.selective_scan(**{**x, "state": st}, done=done, inplace_state=True)
+        _near(y, yr, FWD, "y")
+        _near(st, hr, FWD, "state")
+        y, h = sb.selective_scan(**{**x, "z": None, "state": None, "D": None, "delta_bias": None})
+        yr, hr = orc.scan(**{k: (v.double() if v is not None else None) for k, v in {**x, "z": None, "state": None, "D": None, "delta_bias": None}.items()})
+        _near(y, yr, FWD, "y")
+        _near(h, hr, FWD, "state")
+
+
 def test_scan_reset_at_every_step_and_at_the_first():
     for fill in (lambda d: d.fill_(True), lambda d: d.index_fill_(1, torch.tensor([0], device="cuda"), True),
                  lambda d: d[:, -1].fill_(True)):

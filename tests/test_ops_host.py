@@ -61,6 +61,7 @@ def test_scan_refusals():
     assert f(C.byref(_scan_args(u=L.Rows(0x1002, 1280, 64))), None) == L.ERR_ALIGN
     assert f(C.byref(_scan_args(state_out=0x1008)), None) == L.ERR_ALIGN
     assert f(C.byref(_scan_args(N=1 << 20, D=1 << 20)), None) == L.ERR_SHAPE
+    assert f(C.byref(_scan_args(N=1, L=(1 << 30) + 5)), None) == L.ERR_SHAPE
     assert f(C.byref(_scan_args(N=0)), None) == 0 and f(C.byref(_scan_args(D=0)), None) == 0
     # a long time axis of few channels is cut into pieces, which need scratch
     assert L.load().srwm_b200_scan_scratch_bytes(1, 4096, 64, 16, 1) > 0
