@@ -110,6 +110,8 @@ __global__ void __launch_bounds__(128) conv_fwd_kernel(const ConvParams p) {
 
 // A warp takes 32 quads of channels and p.chunk steps at a time, the block's four warps one chunk after another's; the sums of dw
 // and dbias stay with the threads.  What the outputs behind the chunk give to its inputs comes from K - 1 more steps of dy.
+// An episode's start is read with the rows, AH steps ahead: forward and backward at N 8, L 2048, D 2048 in 16 bits with starts 125 us
+// (132 when each step read its own); without starts 97.
 template <typename T, bool VEC, int K, bool DONE>
 __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
   __shared__ float4 red[4][32];
@@ -129,11 +131,13 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
     const T* py = reinterpret_cast<const T*>(p.dy.p) + n * p.dy.sn + t0 * p.dy.sl + d;
     T* ox = reinterpret_cast<T*>(p.dx.p) + n * p.dx.sn + t0 * p.dx.sl + d;
     Quad<T, VEC> rx[AH], ry[AH], past[K];
+    bool cut[AH];
 #pragma unroll
     for (int j = 1; j < K; ++j) past[j] = input<T, K, VEC>(p, n, t0 - K + j, d, valid);
 #pragma unroll
     for (int k = 0; k < AH; ++k) {
       const int v = t0 + k < p.L && t0 + k < t_all ? valid : 0;
+      if (DONE) cut[k] = v > 0 && starts(p, n, t0 + k);
       rx[k].fetch(px, v);
       ry[k].fetch(py, v);
       px += p.x.sl;
@@ -181,13 +185,14 @@ __global__ void __launch_bounds__(128) conv_bwd_kernel(const ConvParams p) {
         for (int j = 0; j + 1 < K; ++j) acc[j] = acc[j + 1];
         acc[K - 1] = Pairs();
         if (!INNER && last) acc[K - 1] = carried(t);
-        const bool fresh = DONE && t < p.L && starts(p, n, t);
+        const bool fresh = DONE && cut[k];
         if (DONE) age = fresh ? 0 : min(K - 1, age + 1);
 #pragma unroll
         for (int j = 0; j + 1 < K; ++j) win[j] = DONE && fresh ? Pairs() : win[j + 1];
         win[K - 1] = Pairs(rx[k].get());
         Pairs gp(ry[k].get()), a = b;
         const int v = t + AH < p.L && t + AH < t_all ? valid : 0;
+        if (DONE) cut[k] = v > 0 && starts(p, n, t + AH);
         rx[k].fetch(px, v);
         ry[k].fetch(py, v);
         px += p.x.sl;
