@@ -232,6 +232,7 @@ PyObject* scan_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const bool inplace = PyObject_IsTrue(args[11]);
   const bool grad = wants_grad({&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8]});
   if (!scan_ok(s) || (inplace && (grad || !s.state.defined()))) return declined();
+  if (grad) check_capture({&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8]});
   variable_list r;
   {
     NoGil nogil;
@@ -250,7 +251,8 @@ PyObject* conv_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (forward_ad() || !take(args, 0, 2, t) || !take(args, 2, 3, t + 2, true)) return declined();
   const ConvIn s = {t[0], t[1], t[2], t[3], t[4], PyObject_IsTrue(args[5]) != 0};
   const bool inplace = PyObject_IsTrue(args[6]), grad = wants_grad({&t[0], &t[1], &t[2], &t[3]});
-  if (!conv_ok(s) || (inplace && (grad || !s.state.defined()))) return declined();
+  if (!conv_ok(s) || (inplace && (grad || !s.state.defined() || !rows_apart(s.state)))) return declined();
+  if (grad) check_capture({&t[0], &t[1], &t[2], &t[3]});
   variable_list r;
   {
     NoGil nogil;
@@ -272,6 +274,7 @@ PyObject* rms_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (forward_ad() || !take(args, 0, 2, t) || !take(args, 2, 1, &res, true) || !rms_ok(t[0], t[1], res)) return declined();
   const bool grad = wants_grad({&t[0], &t[1], &res});
   if (grad && fp8) return declined();
+  if (grad) check_capture({&t[0], &t[1], &res});
   variable_list r;
   {
     NoGil nogil;

@@ -3,6 +3,9 @@
 #include <algorithm>
 #include <vector>
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <torch/csrc/autograd/variable.h>
+
 #include "host_common.h"
 
 namespace host {
@@ -50,6 +53,26 @@ inline bool fits_int(const Tensor& t) {
   for (const int64_t n : t.sizes())
     if (n > 0x7fffffff) return false;
   return true;
+}
+
+// Rows that can be written in place: no two of [N, L] share a value
+inline bool rows_apart(const Tensor& t) {
+  const int a = t.stride(0) >= t.stride(1) ? 0 : 1, b = 1 - a;      // the rows further apart, and the others
+  return (t.size(b) == 1 || t.stride(b) >= t.size(2)) && (t.size(a) == 1 || t.stride(a) >= (t.size(b) == 1 ? 0 : t.stride(b) * (t.size(b) - 1)) + t.size(2));
+}
+// A leaf's gradient is gathered on the stream on which a graph first used the leaf.  Where that graph still lives and the stream is
+// the default one, a backward pass under capture would draw the default stream into the capture, which ends the process; said
+// here instead, while the forward pass is captured.
+inline void check_capture(std::initializer_list<const Tensor*> ts) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  for (const Tensor* t : ts) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto sum = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = sum ? sum->stream() : std::nullopt;
+    TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(t->device().index()).unwrap(),
+                "a leaf of this call belongs to an autograd graph that was built on the default stream and is still alive: drop its "
+                "outputs (a loss, a carried state) before a training step is captured");
+  }
 }
 
 // ---- selective scan ----

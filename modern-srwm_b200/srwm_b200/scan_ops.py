@@ -22,7 +22,7 @@ with the state carried (no reference operator corresponds; the call conventions 
 
 Rows may be any strided views with a dense last dimension (a time-major ``[L, N, D]`` activation as its transposed view, a slice of
 a wider projection); outputs follow their input's memory order.  Gradients reach every floating argument, the state included, once
-(as with the other recurrences).  ``inplace_state`` (calls without gradients): the new state is written over the given one.
+(as with the other recurrences).  ``inplace_state`` (calls without gradients): the new state is written over the given one (not over an expanded view).
 Sums and states are fp32.  CUDA tensors only; there is no CPU implementation.
 """
 from __future__ import annotations
@@ -109,6 +109,13 @@ def _inplace(state, tensors):
         raise ValueError("inplace_state is for calls without gradients")
 
 
+def _apart(rows):
+    """Whether no two of the rows [N, L, D] share a value."""
+    (far, n), (near, l) = sorted(((rows.stride(i), rows.shape[i]) for i in (0, 1)), reverse=True)
+    width = rows.shape[2]
+    return (l == 1 or near >= width) and (n == 1 or far >= (0 if l == 1 else near * (l - 1)) + width)
+
+
 def _declined(what):
     raise RuntimeError(f"{what}: these tensors cannot be used (forward-mode AD, or a size beyond 2^31)")
 
@@ -164,6 +171,8 @@ def _conv(x, weight, bias, state, done, silu, inplace_state):
         _inplace(state, (x, weight, bias, state))
         if _rows(state) is not state:
             raise ValueError("inplace_state needs a state whose rows are dense")
+        if not _apart(state):
+            raise ValueError("inplace_state needs a state whose rows do not overlap (an expanded view is not written to)")
     if x.numel() == 0:
         if state is None:
             return torch.empty_like(x), torch.zeros(N, K - 1, Dn, device=dev, dtype=dt)

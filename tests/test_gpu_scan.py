@@ -362,3 +362,20 @@ def test_conv_refused_and_empty():
     st = torch.randn(2, 3, 8, device="cuda")
     y, s = sb.causal_conv(x[:, :0], w, state=st)
     assert y.shape == (2, 0, 8) and torch.equal(s, st)
+
+
+def test_conv_state_in_place_is_not_an_expanded_view():
+    x, w = torch.randn(4, 3, 64, device="cuda"), torch.randn(64, 4, device="cuda")
+    with torch.no_grad():
+        for state in (torch.zeros(1, 3, 64, device="cuda").expand(4, -1, -1), torch.zeros(4, 1, 64, device="cuda").expand(-1, 3, -1),
+                      torch.zeros(4 * 64 + 128, device="cuda").as_strided((4, 3, 64), (64, 64, 1))):
+            with pytest.raises(ValueError):
+                sb.causal_conv(x, w, None, state, inplace_state=True)
+            assert not state.any()
+        # rows of a wider buffer, time-major and not, are written, and nothing between them
+        for buf, view in ((torch.randn(4, 5, 96, device="cuda"), lambda b: b[:, 1:4, 16:80]), (torch.randn(3, 6, 64, device="cuda"), lambda b: b[:, 1:5].transpose(0, 1))):
+            y, st = sb.causal_conv(x, w, None, view(buf).clone())
+            got = buf.clone()
+            y2, _ = sb.causal_conv(x, w, None, view(got), inplace_state=True)
+            view(buf).copy_(st)
+            assert torch.equal(y, y2) and torch.equal(got, buf)

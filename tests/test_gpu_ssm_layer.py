@@ -199,3 +199,56 @@ def test_bfloat16_layer_runs():
     assert out.dtype == torch.bfloat16 and st[0].dtype == torch.bfloat16 and st[1].dtype == torch.float32
     grads = torch.autograd.grad(out.float().square().sum(), [h, *layer.parameters()])
     assert all(bool(torch.isfinite(g).all()) for g in grads)
+
+
+def test_capture_beside_a_living_graph_is_refused():
+    """A training step whose leaves belong to a living graph of the default stream is refused while its forward pass is captured; once
+    that graph is gone the step is captured."""
+    u = torch.randn(2, 9, 64, device="cuda")
+    leaves = [torch.randn(64, 4, device="cuda", requires_grad=True), (-torch.rand(64, 16, device="cuda")).requires_grad_(),
+              torch.rand(64, device="cuda").requires_grad_()]
+    B, C = torch.randn(2, 9, 16, device="cuda"), torch.randn(2, 9, 16, device="cuda")
+    ops = [lambda: sb.causal_conv(u, leaves[0])[0], lambda: sb.selective_scan(u, u, leaves[1], B, C)[0], lambda: sb.rms_norm(u, leaves[2])]
+    for leaf, op in zip(leaves, ops):
+        alive = op()
+        want = torch.autograd.grad(alive, leaf, u, retain_graph=True)[0]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match="still alive"):
+                op()
+            keep = u * 2      # (a graph is not empty)
+        del alive, graph, keep
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(op(), leaf, u)[0]
+        graph.replay()
+        assert torch.equal(got, want)
+        del graph
+
+
+def test_layer_under_autocast():
+    """Projections in bfloat16, the norm and the states' types as they are: the carried state of one call fits the next."""
+    layer = _layer(64, 6)
+    h = torch.randn(12, 2, 64, device="cuda")
+    with torch.no_grad():
+        whole = layer(h)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            a, st = layer(h[:5], layer.init_state(2), get_state=True)
+            b, st = layer(h[5:], st, get_state=True)
+    assert st[1].dtype == torch.float32
+    got = torch.cat([a, b]).double()
+    # six results rounded to bf16 in a row (projection, convolution, two projections, scan, projection), half a step of 2^-8 each, and the
+    # products' operands as much again: 12 x 2^-8 of the largest output
+    _near(got, whole.double(), 12 * 2.0 ** -8)
+
+
+def test_states_in_inference_mode():
+    layer = _layer(64, 8)
+    h = torch.randn(4, 3, 64, device="cuda")
+    with torch.no_grad():
+        state = layer.init_state(3)
+        want = [layer(x[None], state, inplace_state=True) for x in h]
+    with torch.inference_mode():
+        state = layer.init_state(3)
+        got = [layer(x[None], state, inplace_state=True) for x in h]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -151,3 +151,21 @@ def test_bucket_clips_on_the_cpu():
     assert abs(float(b.clip_(2.0)) - want) < 1e-5
     assert abs(float(b.flat.norm()) - 2.0) < 1e-5
     assert abs(float(b.clip_(3.0)) - 2.0) < 1e-5 and abs(float(b.flat.norm()) - 2.0) < 1e-5
+
+
+def test_rows_that_share_values():
+    """What an in-place state must not be, against counting the addresses."""
+    from srwm_b200.scan_ops import _apart
+    base = torch.zeros(4096)
+    seen = set()
+    for n, l, d in ((1, 1, 5), (3, 1, 5), (1, 3, 5), (2, 3, 5), (4, 2, 8)):
+        for sn in (0, 1, 4, 5, 8, 10, 15, 16, 20, 64):
+            for sl in (0, 1, 4, 5, 8, 10, 12, 20, 32):
+                rows = base.as_strided((n, l, d), (sn, sl, 1))
+                where = [i * sn + j * sl + k for i in range(n) for j in range(l) for k in range(d)]
+                apart = len(set(where)) == len(where)
+                seen.add(apart)
+                assert not _apart(rows) or apart, (n, l, d, sn, sl)              # never a race
+                if sn % max(sl, 1) == 0 or sl % max(sn, 1) == 0:                 # and every nested order that there is
+                    assert _apart(rows) == apart or (min(sn, sl) < d and n > 1 and l > 1), (n, l, d, sn, sl)
+    assert seen == {True, False}
