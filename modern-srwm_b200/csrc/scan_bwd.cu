@@ -403,7 +403,7 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
               const u64 d2 = dup2(x[c].x), x2 = dup2(x[c].y);
 #pragma unroll
               for (int i = 0; i < NP; ++i) {
-                a[k][c][i] = exp2_pair(mul2(d2, A2[c][i]));
+                a[k][c][i] = decay2(d2, A2[c][i]);
                 in[k][c][i] = mul2(x2, b2[i]);
               }
             }
@@ -429,7 +429,7 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
             const u64 d2 = dup2(x[c].x), x2 = dup2(x[c].y);
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-              a[k][c][i] = exp2_pair(mul2(d2, A2[c][i]));
+              a[k][c][i] = decay2(d2, A2[c][i]);
               ah[k][c][i] = mul2(x2, b2[i]);
             }
           }
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(BwdCarryShape<S>::NT) scan_bwd_carry_kernel(co
           sum_d[c] += x[c].x;
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
-            const u64 g = fma2<true>(c2[i], g2, gc[c][i]), a = exp2_pair(mul2(d2, A2[c][i]));
+            const u64 g = fma2<true>(c2[i], g2, gc[c][i]), a = decay2(d2, A2[c][i]);
             gc[c][i] = fresh ? 0ull : mul2(a, g);
           }
         }
@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(BwdCarryShape<S>::NT) scan_bwd_carry_kernel(co
     if (c >= mine) continue;
     u64 decay[NP];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) decay[i] = cut ? 0ull : exp2_pair(mul2(dup2(sum_d[c]), A2[c][i]));
+    for (int i = 0; i < NP; ++i) decay[i] = cut ? 0ull : decay2(dup2(sum_d[c]), A2[c][i]);
     store_states<Sh>(p.carry + (2 * seg - 2) * states + own + c * S, q, gc[c]);
     store_states<Sh>(p.carry + (2 * seg - 1) * states + own + c * S, q, decay);
   }

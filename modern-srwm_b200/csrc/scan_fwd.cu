@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 && C == 2 
             if (CARRY && (WHOLE || t < steps)) sum_d[c] += x[c].x;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-              a[b][k][c][i] = exp2_pair(mul2(d2, A2[c][i]));
+              a[b][k][c][i] = decay2(d2, A2[c][i]);
               in[b][k][c][i] = mul2(x2, b2[i]);
             }
           }
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 && C == 2 
     if (CARRY) {
       u64 decay[NP];
 #pragma unroll
-      for (int i = 0; i < NP; ++i) decay[i] = cut ? 0ull : exp2_pair(mul2(dup2(sum_d[c]), A2[c][i]));
+      for (int i = 0; i < NP; ++i) decay[i] = cut ? 0ull : decay2(dup2(sum_d[c]), A2[c][i]);
       store_states<Sh>(p.carry + (2 * seg + 1) * states + o, q, h[c]);
       store_states<Sh>(p.carry + (2 * seg + 2) * states + o, q, decay);
     } else if (seg == p.nseg - 1 && p.hT) {
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(Shape<S, 1, SCAN_TILE>::WALK) scan_step_kernel
       u64 acc = 0ull;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        u64 a = exp2_pair(mul2(dup2(db), A2[i]));
+        u64 a = decay2(dup2(db), A2[i]);
         if (fresh[b]) a = h[b][i] = 0ull;
         h[b][i] = fma2<true>(a, h[b][i], mul2(dup2(xb), b2[b][i]));
         acc = i == 0 ? mul2(h[b][i], c2[b][i]) : fma2<true>(h[b][i], c2[b][i], acc);
