@@ -379,3 +379,18 @@ def test_conv_state_in_place_is_not_an_expanded_view():
             y2, _ = sb.causal_conv(x, w, None, view(got), inplace_state=True)
             view(buf).copy_(st)
             assert torch.equal(y, y2) and torch.equal(got, buf)
+
+
+@pytest.mark.parametrize("S", [8, 16, 32, 64])
+@pytest.mark.parametrize("L,D", [(1, 96), (37, 96), (2000, 36)])
+def test_steps_of_no_length_leave_the_state(S, L, D):
+    """Delta of zero (a padded step) keeps every bit of the state and of its gradient, in one piece of the time axis or several."""
+    g = torch.Generator(device="cuda").manual_seed(S + L)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)      # noqa: E731
+    u, B, C, A = rand(2, L, D), rand(2, L, S), rand(2, L, S), -torch.rand(D, S, device="cuda", generator=g) * S
+    state, go = rand(2, D, S).requires_grad_(), rand(2, D, S)
+    with torch.no_grad():
+        assert torch.equal(sb.selective_scan(u, torch.zeros_like(u), A, B, C, state=state, delta_softplus=False)[1], state)
+    _, last = sb.selective_scan(u, torch.zeros_like(u), A, B, C, state=state, delta_softplus=False)
+    assert torch.equal(last, state)
+    assert torch.equal(torch.autograd.grad(last, state, go)[0], go)
