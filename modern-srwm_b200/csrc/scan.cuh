@@ -246,6 +246,17 @@ __device__ __forceinline__ u64 decay2(u64 delta, u64 A) {
   return pack2(ex2(a), ex2(b));
 }
 
+// The state (or its gradient) on the far side of a piece of the time axis, from the one on this side, what the piece adds and the product of
+// its decays.  Where an episode begins inside the piece nothing goes through, not even a NaN or an infinity: such a piece leaves CUT as its
+// product, a zero that no exponential gives (a product of decays may well be +0).
+constexpr u64 CUT = 0x8000000080000000ull;      // a pair of -0
+template <int NP>
+__device__ __forceinline__ void through_piece(u64 (&h)[NP], const u64 (&decay)[NP], const u64 (&end)[NP]) {
+  const bool cut = decay[0] == CUT;
+#pragma unroll
+  for (int k = 0; k < NP; ++k) h[k] = cut ? end[k] : fma2<true>(decay[k], h[k], end[k]);
+}
+
 // Where a CTA works: sequence, group, first channel, channels of the group from there on
 template <int CH>
 struct Place {

@@ -147,8 +147,7 @@ __global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 && C == 2 
         u64 decay[NP], end[NP];
         load_states<Sh>(p.carry + (2 * i + 1) * states + o, q, end);
         load_states<Sh>(p.carry + (2 * i + 2) * states + o, q, decay);
-#pragma unroll
-        for (int k = 0; k < NP; ++k) h[c][k] = fma2<true>(decay[k], h[c][k], end[k]);
+        through_piece(h[c], decay, end);
       }
     }
 #pragma unroll
@@ -241,7 +240,7 @@ __global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 && C == 2 
     if (CARRY) {
       u64 decay[NP];
 #pragma unroll
-      for (int i = 0; i < NP; ++i) decay[i] = cut ? 0ull : decay2(dup2(sum_d[c]), A2[c][i]);
+      for (int i = 0; i < NP; ++i) decay[i] = cut ? CUT : decay2(dup2(sum_d[c]), A2[c][i]);
       store_states<Sh>(p.carry + (2 * seg + 1) * states + o, q, h[c]);
       store_states<Sh>(p.carry + (2 * seg + 2) * states + o, q, decay);
     } else if (seg == p.nseg - 1 && p.hT) {

@@ -394,3 +394,37 @@ def test_steps_of_no_length_leave_the_state(S, L, D):
     _, last = sb.selective_scan(u, torch.zeros_like(u), A, B, C, state=state, delta_softplus=False)
     assert torch.equal(last, state)
     assert torch.equal(torch.autograd.grad(last, state, go)[0], go)
+
+
+# ---- values that are not finite, and a time axis that is cut into pieces ----
+
+def _pieces(L, D, S):
+    """The case's time axis is cut into three pieces at least: the forward's scratch is (2 pieces - 1) states."""
+    from srwm_b200 import _lib
+    return (_lib.load().srwm_b200_scan_scratch_bytes(2, L, D, S, 1) // (4 * 2 * D * S) + 1) // 2
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("S", [8, 16, 32, 64])
+@pytest.mark.parametrize("L,D,at,reset", [(1000, 64, 300, 700), (512, 33, 10, 500)])
+def test_scan_bad_values_do_not_pass_a_reset_in_another_piece(L, D, at, reset, S, bad):
+    """NaN and infinities of an episode, pieces in front of the next one's start, leave every bit of what follows."""
+    assert _pieces(L, D, S) >= 3
+    x, _, _, _ = _inputs(2, L, D, S, 1, torch.float32, seed=30)
+    done = torch.zeros(2, L, dtype=torch.bool, device="cuda")
+    done[0, reset] = True
+    spoilt = {**x, "u": x["u"].clone()}
+    spoilt["u"][0, at] = bad
+    first = done.clone()
+    first[0, 0] = True
+    recycled = {**x, "state": x["state"].clone()}
+    recycled["state"][0] = bad
+    for grad in (False, True):      # (the second keeps states for a backward)
+        with torch.set_grad_enabled(grad):
+            clean = sb.selective_scan(**{**x, "A": x["A"].detach().requires_grad_(grad)}, done=done)
+            y, h = sb.selective_scan(**{**spoilt, "A": x["A"].detach().requires_grad_(grad)}, done=done)
+            assert torch.equal(y[0, :at], clean[0][0, :at]) and not bool(torch.isfinite(y[0, at]).any())
+            assert torch.equal(y[0, reset:], clean[0][0, reset:]) and torch.equal(y[1], clean[0][1]) and torch.equal(h, clean[1])
+            clean = sb.selective_scan(**{**x, "A": x["A"].detach().requires_grad_(grad)}, done=first)
+            y, h = sb.selective_scan(**{**recycled, "A": x["A"].detach().requires_grad_(grad)}, done=first)
+            assert torch.equal(y, clean[0]) and torch.equal(h, clean[1])
