@@ -315,8 +315,7 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
       u64 decay[NP], end[NP];
       load_turned<Sh>(p.carry + (2 * i - 2) * states + o, q, order, end);
       load_turned<Sh>(p.carry + (2 * i - 1) * states + o, q, order, decay);
-#pragma unroll
-      for (int k = 0; k < NP; ++k) gc[c][k] = fma2<true>(decay[k], gc[c][k], end[k]);
+      through_piece(gc[c], decay, end);
     }
   }
   // in part[][][][]: of v[0] of sum_groups (ST 4: of the step that the lane keeps)
@@ -671,7 +670,7 @@ __global__ void __launch_bounds__(BwdCarryShape<S>::NT) scan_bwd_carry_kernel(co
     if (c >= mine) continue;
     u64 decay[NP];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) decay[i] = cut ? 0ull : decay2(dup2(sum_d[c]), A2[c][i]);
+    for (int i = 0; i < NP; ++i) decay[i] = cut ? CUT : decay2(dup2(sum_d[c]), A2[c][i]);
     store_states<Sh>(p.carry + (2 * seg - 2) * states + own + c * S, q, gc[c]);
     store_states<Sh>(p.carry + (2 * seg - 1) * states + own + c * S, q, decay);
   }

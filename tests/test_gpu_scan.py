@@ -428,3 +428,34 @@ def test_scan_bad_values_do_not_pass_a_reset_in_another_piece(L, D, at, reset, S
             clean = sb.selective_scan(**{**x, "A": x["A"].detach().requires_grad_(grad)}, done=first)
             y, h = sb.selective_scan(**{**recycled, "A": x["A"].detach().requires_grad_(grad)}, done=first)
             assert torch.equal(y, clean[0]) and torch.equal(h, clean[1])
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("S", [8, 16, 32, 64])
+@pytest.mark.parametrize("L,D,at,reset", [(1000, 64, 900, 400), (512, 33, 500, 100)])
+def test_scan_bad_gradients_do_not_pass_a_reset_in_another_piece(L, D, at, reset, S, bad):
+    """A gradient of an output or of the last state that is NaN or infinite, and inputs that are, leave every bit of the rows' gradients
+    in the episodes in front (behind)."""
+    assert _pieces(L, D, S) >= 3
+    x, _, gy, gs = _inputs(2, L, D, S, 1, torch.float32, seed=31)
+    done = torch.zeros(2, L, dtype=torch.bool, device="cuda")
+    done[0, reset] = True
+    rows = ("u", "delta", "B", "C", "z")
+
+    def grads(gy, gs, **change):
+        args = {k: v.detach().requires_grad_() for k, v in {**x, **change}.items()}
+        return dict(zip(NAMES, torch.autograd.grad(list(sb.selective_scan(**args, done=done)), [args[k] for k in NAMES], [gy, gs])))
+    clean = grads(gy, gs)
+    assert all(bool(torch.isfinite(v).all()) for v in clean.values())
+    gy_bad, gs_bad, u_bad = gy.clone(), gs.clone(), x["u"].clone()
+    gy_bad[0, at] = bad
+    gs_bad[0] = bad
+    for got in (grads(gy_bad, gs), grads(gy, gs_bad)):
+        for k in rows:
+            assert torch.equal(got[k][0, :reset], clean[k][0, :reset]) and torch.equal(got[k][1], clean[k][1]), k
+        assert torch.equal(got["state"], clean["state"]) and not bool(torch.isfinite(got["B"][0, at]).any())
+    u_bad[0, reset // 2] = bad
+    got = grads(gy, gs, u=u_bad)
+    for k in rows:
+        assert torch.equal(got[k][0, reset:], clean[k][0, reset:]) and torch.equal(got[k][1], clean[k][1]), k
+    assert torch.equal(got["state"], clean["state"])
