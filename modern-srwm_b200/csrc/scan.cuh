@@ -246,15 +246,23 @@ __device__ __forceinline__ u64 decay2(u64 delta, u64 A) {
   return pack2(ex2(a), ex2(b));
 }
 
-// The state (or its gradient) on the far side of a piece of the time axis, from the one on this side, what the piece adds and the product of
-// its decays.  Where an episode begins inside the piece nothing goes through, not even a NaN or an infinity: such a piece leaves CUT as its
-// product, a zero that no exponential gives (a product of decays may well be +0).
+// The state (or its gradient) on the far side of a piece of the time axis, from the one on this side, what the piece adds and the square root of
+// the product of its decays: steps as given may be negative, and a piece's growth (or decay) be beyond a float where what it makes of a small
+// state is not.  A state of zero stays zero through any growth.  Where an episode begins inside the piece nothing goes through, not even a NaN
+// or an infinity: such a piece leaves CUT, a zero that no exponential gives, and is told by it (a product of decays may well be +0).
 constexpr u64 CUT = 0x8000000080000000ull;      // a pair of -0
+__device__ __forceinline__ u64 piece_root(float sum_d, u64 A) { return decay2(dup2(0.5f * sum_d), A); }
 template <int NP>
-__device__ __forceinline__ void through_piece(u64 (&h)[NP], const u64 (&decay)[NP], const u64 (&end)[NP]) {
-  const bool cut = decay[0] == CUT;
+__device__ __forceinline__ void through_piece(u64 (&h)[NP], const u64 (&root)[NP], const u64 (&end)[NP]) {
+  const bool cut = root[0] == CUT;
 #pragma unroll
-  for (int k = 0; k < NP; ++k) h[k] = cut ? end[k] : fma2<true>(decay[k], h[k], end[k]);
+  for (int k = 0; k < NP; ++k) {
+    float h0, h1, n0, n1, e0, e1;
+    unpack2(h[k], h0, h1);
+    unpack2(fma2<true>(root[k], mul2(root[k], h[k]), end[k]), n0, n1);
+    unpack2(end[k], e0, e1);
+    h[k] = pack2(cut || h0 == 0.f ? e0 : n0, cut || h1 == 0.f ? e1 : n1);
+  }
 }
 
 // Where a CTA works: sequence, group, first channel, channels of the group from there on

@@ -25,7 +25,7 @@ struct ScanParams {
   const uint8_t* done;
   long long done_n, done_l;
   float* ckpt;                  // [N][ceil(L / SCAN_CKPT)][D][S], the state in front of each eighth step
-  float* carry;                 // nseg > 1: each piece's end from zero and the product of its decays, [N][D][S] each (forward: the first state in front)
+  float* carry;                 // nseg > 1: each piece's end from zero and the product of its decays (its root), [N][D][S] each (forward: the first state in front)
   // backward
   ScanRows dy, du, ddelta, dz, dB, dC;
   const float* dhT;

@@ -312,10 +312,10 @@ __device__ __forceinline__ void scan_bwd_walk(const ScanParams& p, BwdSmem<S>& s
     if (p.dhT) load_turned<Sh>(p.dhT + o, q, order, gc[c]);
 #pragma unroll 4
     for (int i = p.nseg - 1; i > seg; --i) {      // the pieces behind, the last first
-      u64 decay[NP], end[NP];
+      u64 root[NP], end[NP];
       load_turned<Sh>(p.carry + (2 * i - 2) * states + o, q, order, end);
-      load_turned<Sh>(p.carry + (2 * i - 1) * states + o, q, order, decay);
-      through_piece(gc[c], decay, end);
+      load_turned<Sh>(p.carry + (2 * i - 1) * states + o, q, order, root);
+      through_piece(gc[c], root, end);
     }
   }
   // in part[][][][]: of v[0] of sum_groups (ST 4: of the step that the lane keeps)
@@ -668,11 +668,11 @@ __global__ void __launch_bounds__(BwdCarryShape<S>::NT) scan_bwd_carry_kernel(co
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     if (c >= mine) continue;
-    u64 decay[NP];
+    u64 root[NP];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) decay[i] = cut ? CUT : decay2(dup2(sum_d[c]), A2[c][i]);
+    for (int i = 0; i < NP; ++i) root[i] = cut ? CUT : piece_root(sum_d[c], A2[c][i]);
     store_states<Sh>(p.carry + (2 * seg - 2) * states + own + c * S, q, gc[c]);
-    store_states<Sh>(p.carry + (2 * seg - 1) * states + own + c * S, q, decay);
+    store_states<Sh>(p.carry + (2 * seg - 1) * states + own + c * S, q, root);
   }
 }
 

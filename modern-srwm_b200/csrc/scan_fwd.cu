@@ -144,10 +144,10 @@ __global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 && C == 2 
       load_states<Sh>(p.carry + o, q, h[c]);
 #pragma unroll 4
       for (int i = 0; i < seg; ++i) {     // the pieces in front, in order
-        u64 decay[NP], end[NP];
+        u64 root[NP], end[NP];
         load_states<Sh>(p.carry + (2 * i + 1) * states + o, q, end);
-        load_states<Sh>(p.carry + (2 * i + 2) * states + o, q, decay);
-        through_piece(h[c], decay, end);
+        load_states<Sh>(p.carry + (2 * i + 2) * states + o, q, root);
+        through_piece(h[c], root, end);
       }
     }
 #pragma unroll
@@ -238,11 +238,11 @@ __global__ void __launch_bounds__(Shape<S, C, SCAN_TILE>::NT, S == 64 && C == 2 
     if (c >= mine) continue;
     const long long o = own + c * S;
     if (CARRY) {
-      u64 decay[NP];
+      u64 root[NP];
 #pragma unroll
-      for (int i = 0; i < NP; ++i) decay[i] = cut ? CUT : decay2(dup2(sum_d[c]), A2[c][i]);
+      for (int i = 0; i < NP; ++i) root[i] = cut ? CUT : piece_root(sum_d[c], A2[c][i]);
       store_states<Sh>(p.carry + (2 * seg + 1) * states + o, q, h[c]);
-      store_states<Sh>(p.carry + (2 * seg + 2) * states + o, q, decay);
+      store_states<Sh>(p.carry + (2 * seg + 2) * states + o, q, root);
     } else if (seg == p.nseg - 1 && p.hT) {
       store_states<Sh>(p.hT + o, q, h[c]);
     }

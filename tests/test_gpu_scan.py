@@ -459,3 +459,58 @@ def test_scan_bad_gradients_do_not_pass_a_reset_in_another_piece(L, D, at, reset
     for k in rows:
         assert torch.equal(got[k][0, reset:], clean[k][0, reset:]) and torch.equal(got[k][1], clean[k][1]), k
     assert torch.equal(got["state"], clean["state"])
+
+
+@pytest.mark.parametrize("S", [8, 16, 32, 64])
+def test_scan_growth_that_a_float_does_not_hold_over_a_piece(S):
+    """Steps as given may be negative, and a state grow.  A state of zero stays zero however much a whole piece grows, and a small one comes
+    to what its steps make of it, as long as these are finite; its gradient likewise.  Of the largest value: 140 steps of growth and
+    decay, 1.5 x 2^-22 each, 5e-5, and three times that for gradients.  A piece's product has its steps' sum in fp32 as well, here up to
+    98 in 70 additions, half-steps of 2^-18 for 24 of them, 2^-19 for 23, 2^-20 for 11 and less: 1.5e-4 in all."""
+    N, L, D = 2, 1000, 64
+    assert _pieces(L, D, S) == 13      # of 80 steps
+    x, _, gy, gs = _inputs(N, L, D, S, 1, torch.float32, seed=32)
+    x["delta_bias"] = None
+    x["delta"] = torch.full((N, L, D), 1.4, device="cuda")
+    x["A"] = torch.full((D, S), -1.0, device="cuda")
+
+    def both(x, gy, gs):
+        names = [k for k in NAMES if x[k] is not None]
+        ref = {k: (v if v is None else v.detach().double().requires_grad_()) for k, v in x.items()}
+        args = {k: (v if v is None else v.detach().requires_grad_()) for k, v in x.items()}
+        want, got = orc.scan(**ref, softplus=False), sb.selective_scan(**args, delta_softplus=False)
+        gw = torch.autograd.grad(list(want), [ref[k] for k in names], [gy.double(), gs.double()])
+        gg = torch.autograd.grad(list(got), [args[k] for k in names], [gy, gs])
+        return [(a.detach(), b.detach()) for a, b in zip(got, want)], {k: (a, b) for k, a, b in zip(names, gg, gw)}
+
+    # nothing in front of step 400, and growth beyond every float: 2^323 in each of the pieces from 160 to 320
+    empty = {**x, "state": None, "u": x["u"].clone(), "delta": x["delta"].clone()}
+    empty["u"][:, :400] = 0.0
+    empty["delta"][:, 160:320] = -2.8
+    out, grads = both(empty, gy * (torch.arange(L, device="cuda") >= 400)[:, None], gs)
+    for a, b in out:
+        _near(a, b, 5e-5)
+    for k in ("B", "C", "z"):      # (of u and delta, those of the steps in front of the growth are beyond a float themselves)
+        _near(grads[k][0][:, 400:], grads[k][1][:, 400:], 1.5e-4, k)
+    # a small state through 98 e-folds inside one piece, and as many back
+    small = {**x, "state": 1e-30 * x["state"], "u": torch.zeros_like(x["u"]), "delta": x["delta"].clone()}
+    small["delta"][:, :160] = 0.0
+    small["delta"][:, 160:230] = -1.4
+    small["delta"][:, 230:330] = 0.0
+    out, _ = both(small, gy, gs)
+    _near(*out[0], 2e-4)
+    _near(out[0][0][:, 240:330], out[0][1][:, 240:330], 2e-4)
+    assert 1e11 < float(out[0][1].abs().max()) < 1e16
+    # a small gradient, the same way back
+    last = {**x, "u": x["u"].clone(), "delta": x["delta"].clone()}
+    last["u"][:, 500:] = 0.0
+    last["delta"][:, 800:870] = -1.4
+    last["delta"][:, 870:] = 0.0
+    last["delta"][:, 700:800] = 1e-3
+    out, grads = both(last, gy * (torch.arange(L, device="cuda") < 500)[:, None], 1e-30 * gs)
+    for a, b in out:
+        _near(a, b, 5e-5)
+    for k in ("u", "state"):
+        _near(*grads[k], 3e-4, k)
+    _near(grads["u"][0][:, 700:800], grads["u"][1][:, 700:800], 3e-4, "in front of the growth")
+    assert 1e11 < float(grads["u"][1][:, 500:].abs().max()) < 1e16
