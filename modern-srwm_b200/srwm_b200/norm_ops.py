@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from .scan_ops import _declined, _like, _tensor
+from .scan_ops import _declined, _empty, _like, _tensor
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
@@ -42,8 +42,8 @@ def _checked(x, weight, residual, eps, fp8):
         raise ValueError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
     if x.numel() == 0:
         y = (torch.empty_like(x, dtype=torch.float8_e4m3fn), x.new_empty((*x.shape[:-1], 1), dtype=torch.float32)) if fp8 \
-            else (torch.empty_like(x),)
-        y += () if residual is None else (torch.empty_like(x),)
+            else (_empty(torch.empty_like(x.detach()), x, weight, residual),)
+        y += () if residual is None else (_empty(torch.empty_like(x.detach()), x, residual),)
         return y if len(y) > 1 else y[0]
     r = L.host().rms_norm(x.contiguous(), weight.contiguous(), None if residual is None else residual.contiguous(), eps, fp8)
     return _declined("rms_norm") if r is NotImplemented else r

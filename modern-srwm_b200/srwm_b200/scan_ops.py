@@ -116,6 +116,14 @@ def _apart(rows):
     return (l == 1 or near >= width) and (n == 1 or far >= (0 if l == 1 else near * (l - 1)) + width)
 
 
+def _empty(out, *tensors):
+    """An output without values: all of ``tensors`` have a gradient through it, zeros."""
+    for t in tensors:
+        if torch.is_grad_enabled() and t is not None and t.requires_grad:
+            out = out + 0 * t.sum().to(out.dtype)
+    return out
+
+
 def _declined(what):
     raise RuntimeError(f"{what}: these tensors cannot be used (forward-mode AD, or a size beyond 2^31)")
 
@@ -147,9 +155,10 @@ def _scan(u, delta, A, B, C, D, z, delta_bias, state, done, delta_softplus, inpl
         if not state.is_contiguous() or state.data_ptr() % 16:
             raise ValueError("inplace_state needs a dense state on a 16-byte boundary")
     if u.numel() == 0:      # nothing to run: the state is carried through unchanged
+        y = _empty(torch.empty_like(u.detach()), u, delta, A, B, C, D, z, delta_bias, state)
         if state is None:
-            return torch.empty_like(u), torch.zeros(N, Dn, S, device=dev)
-        return torch.empty_like(u), state if inplace_state else state.clone()
+            return y, torch.zeros(N, Dn, S, device=dev)
+        return y, state if inplace_state else state.clone()
     r = L.host().selective_scan(_rows(u), _rows(delta), _dense(A), _rows(B), _rows(C), _dense(D), _rows(z), _dense(delta_bias),
                                 state if inplace_state else _dense(state), done, delta_softplus, inplace_state)
     return _declined("selective_scan") if r is NotImplemented else r
@@ -174,8 +183,9 @@ def _conv(x, weight, bias, state, done, silu, inplace_state):
         if not _apart(state):
             raise ValueError("inplace_state needs a state whose rows do not overlap (an expanded view is not written to)")
     if x.numel() == 0:
+        y = _empty(torch.empty_like(x.detach()), x, weight, bias, state)
         if state is None:
-            return torch.empty_like(x), torch.zeros(N, K - 1, Dn, device=dev, dtype=dt)
-        return torch.empty_like(x), state if inplace_state else state.clone()
+            return y, torch.zeros(N, K - 1, Dn, device=dev, dtype=dt)
+        return y, state if inplace_state else state.clone()
     r = L.host().causal_conv(_rows(x), _dense(weight), _dense(bias), _rows(state), done, silu, inplace_state)
     return _declined("causal_conv") if r is NotImplemented else r

@@ -252,3 +252,39 @@ def test_states_in_inference_mode():
         state = layer.init_state(3)
         got = [layer(x[None], state, inplace_state=True) for x in h]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("N,L", [(0, 5), (3, 0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_calls_without_values_have_gradients(N, L, dtype):
+    """A rank without sequences, an unroll without steps: every argument has a gradient, zeros, and a state its output's."""
+    rows = lambda w: torch.randn(N, L, w, device="cuda", dtype=dtype, requires_grad=True)      # noqa: E731
+    par = lambda *s: torch.randn(*s, device="cuda", requires_grad=True)      # noqa: E731
+    u, delta, z, B, C, state = rows(32), rows(32), rows(32), rows(16), rows(16), par(N, 32, 16)
+    leaves = [u, delta, par(32, 16), B, C, par(32), z, par(32), state]
+    with torch.no_grad():
+        leaves[2][0, 0] = float("inf")
+    y, h = sb.selective_scan(*leaves)
+    gs = torch.randn_like(h)
+    grads = torch.autograd.grad([y, h], leaves, [torch.empty_like(y), gs])
+    assert y.shape == (N, L, 32) and all(g.shape == t.shape and not bool(g.any()) for g, t in zip(grads[:-1], leaves)) and torch.equal(grads[-1], gs)
+    y = sb.selective_scan(*leaves[:5])[0]
+    assert all(not bool(g.any()) for g in torch.autograd.grad(y, leaves[:5], torch.empty_like(y)))
+    window = torch.randn(N, 3, 32, device="cuda", dtype=dtype, requires_grad=True)
+    leaves = [u, par(32, 4), par(32), window]
+    y, h = sb.causal_conv(*leaves)
+    gs = torch.randn_like(h)
+    grads = torch.autograd.grad([y, h], leaves, [torch.empty_like(y), gs])
+    assert y.shape == (N, L, 32) and not any(bool(g.any()) for g in grads[:-1]) and torch.equal(grads[-1], gs)
+    w = par(32)
+    y, s = sb.rms_norm(u, w, residual=z)
+    assert not any(bool(g.any()) for g in torch.autograd.grad([y, s], [u, z, w], [torch.empty_like(y), torch.empty_like(s)]))
+    y = sb.rms_norm(u, w)
+    assert y.requires_grad and not bool(torch.autograd.grad(y, w, torch.empty_like(y))[0].any())
+    with torch.no_grad():
+        assert not sb.rms_norm(u, w).requires_grad and not sb.selective_scan(u, delta, leaves[1].new_zeros(32, 16), B, C)[0].requires_grad
+    layer = _layer(32, 4).to(dtype)
+    h = torch.randn(L, N, 32, device="cuda", dtype=dtype, requires_grad=True)
+    out, st = layer(h, layer.init_state(N), torch.zeros(L, N, dtype=torch.bool, device="cuda"), get_state=True, residual=h)
+    assert out.shape == (L, N, 32) and st[0].shape == (N, 3, 64) and st[1].shape == (N, 64, 16)
+    assert not any(bool(g.any()) for g in torch.autograd.grad(out.sum(), [h, *layer.parameters()]))
