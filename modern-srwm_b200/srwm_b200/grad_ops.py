@@ -49,6 +49,47 @@ def clip_tensors_(grads, max_norm, error_if_nonfinite=False):
     return _checked(grads, max_norm) if r is NotImplemented else r
 
 
+def _bytes(t):
+    """[(distance, count)] of a tensor's bytes, the largest distance first."""
+    dims = [(st * t.element_size(), n) for st, n in zip(t.stride(), t.shape) if n > 1] + [(1, t.element_size())]
+    return sorted(dims, reverse=True)
+
+
+def _meet(delta, dims):
+    """Whether sum_k d_k distance_k = delta for some d_k from low_k to high_k; dims: (distance, low, high), the largest distance first."""
+    if not dims:
+        return delta == 0
+    (st, low, high), rest = dims[0], dims[1:]
+    if st == 0:
+        return _meet(delta, rest)
+    first = max(low, -((sum(s * h for s, _, h in rest) - delta) // st))
+    last = min(high, (delta - sum(s * l for s, l, _ in rest)) // st)
+    return any(_meet(delta - d * st, rest) for d in range(first, last + 1))
+
+
+def _overlap(tensors):
+    """Whether a byte belongs to two values of these tensors (of one of them, where its dimensions are not nested, is taken to)."""
+    spans = []
+    for t in tensors:
+        if t.numel() == 0:
+            continue
+        dims, extent = _bytes(t), 0
+        for st, n in reversed(dims):
+            if st <= extent:
+                return True
+            extent += st * (n - 1)
+        spans.append((t.data_ptr(), t.data_ptr() + extent, dims))
+    spans.sort(key=lambda s: s[:2])
+    for i, (a, end, da) in enumerate(spans):
+        for b, _, db in spans[i + 1:]:
+            if b > end:
+                break
+            both = [(st, 0, n - 1) for st, n in da] + [(st, 1 - n, 0) for st, n in db]
+            if _meet(b - a, sorted(both, reverse=True)):
+                return True
+    return False
+
+
 @torch.no_grad()
 def _checked(tensors, max_norm):
     device = tensors[0].device
@@ -63,6 +104,8 @@ def _checked(tensors, max_norm):
         if t.layout is not torch.strided:
             raise TypeError("gradients must be dense tensors")
     plain = [t.detach().as_subclass(torch.Tensor) for t in tensors]
+    if max_norm >= 0.0 and _overlap(plain):
+        raise ValueError("gradients overlap in memory (the same one twice, views of one another or an expanded one)")
     dense = [t.contiguous() for t in plain]      # (the same memory where it is dense already)
     r = L.host().grads_norm(dense, max_norm, False)
     if r is NotImplemented:

@@ -196,3 +196,22 @@ def test_clip_refused_and_the_bucket():
     b.view(0).fill_(3.0)
     b.view(1).fill_(-4.0)
     assert abs(float(b.clip_(2.0)) - (9.0 * 6 + 16.0 * 5) ** 0.5) < 1e-5 and abs(float(b.flat.norm()) - 2.0) < 1e-5
+
+
+def test_clip_of_views_that_share_values():
+    """Views with gaps that overlap are refused before anything is scaled; those side by side in one buffer are scaled."""
+    wide, dense = torch.randn(40, 41, device="cuda"), torch.randn(50, device="cuda")
+    for grads in ([dense, wide[:, 1:20], wide[:, 1:20]], [wide[:, :20], wide[:, 19:], dense], [wide[:, 3], wide], [dense, wide[:1].expand(3, -1)]):
+        keep, rest = wide.clone(), dense.clone()
+        with pytest.raises(ValueError, match="overlap"):
+            sb.grad_ops.clip_tensors_(grads, 1.0)
+        ps = [torch.nn.Parameter(torch.empty(g.shape, device="cuda")) for g in grads]
+        for p, g in zip(ps, grads):
+            p.grad = g
+        with pytest.raises(ValueError, match="overlap"):
+            sb.clip_grad_norm_(ps, 1.0)
+        assert torch.equal(wide, keep) and torch.equal(dense, rest)
+    norm, want = orc.clip([wide], 0.5)
+    got = sb.grad_ops.clip_tensors_([wide[:, 20:], wide[:, :20:2], wide[:, 1:20:2]], 0.5)
+    assert abs(float(got) / float(norm) - 1) < 1e-6
+    _near(wide, want[0], 1.5e-6)

@@ -169,3 +169,31 @@ def test_rows_that_share_values():
                 if sn % max(sl, 1) == 0 or sl % max(sn, 1) == 0:                 # and every nested order that there is
                     assert _apart(rows) == apart or (min(sn, sl) < d and n > 1 and l > 1), (n, l, d, sn, sl)
     assert seen == {True, False}
+
+
+def test_gradients_that_share_values():
+    """What clipping must not be given, against counting the bytes: no overlap is missed, and only a tensor whose own dimensions are not
+    nested is taken to overlap without one."""
+    import random
+    from srwm_b200.grad_ops import _overlap
+    base, rng, found = torch.zeros(4096), random.Random(1), 0
+    for _ in range(2000):
+        ts, where = [], []
+        for _ in range(rng.choice((1, 2, 2, 3))):
+            d, dtype = rng.choice((0, 1, 2, 3)), rng.choice((torch.float32, torch.bfloat16))
+            shape, strides = [rng.choice((1, 2, 3, 4)) for _ in range(d)], [rng.choice((0, 1, 1, 2, 3, 4, 6, 8, 12, 24, 48)) for _ in range(d)]
+            t = base.view(dtype).as_strided(shape, strides, rng.randrange(0, 60))
+            ts.append(t)
+            offsets = [t.storage_offset()]
+            for n, st in zip(shape, strides):
+                offsets = [o + i * st for o in offsets for i in range(n)]
+            where += [o * t.element_size() + j for o in offsets for j in range(t.element_size())]
+        shared = len(set(where)) != len(where)
+        found += shared
+        assert _overlap(ts) or not shared, ts
+        assert shared or not _overlap(ts) or any(_overlap([t]) for t in ts), ts
+    assert 500 < found < 1500
+    wide = torch.zeros(40, 41)
+    assert not _overlap([wide[:, :20], wide[:, 20:], torch.zeros(0)]) and not _overlap([wide[:, ::2], wide[:, 1::2]]) and not _overlap([wide[3:5].t(), wide[5:]])
+    assert _overlap([wide[:, :20], wide[:, 19:]]) and _overlap([wide[:, ::2], wide[:, ::2]]) and _overlap([wide[:, 3], wide])
+    assert _overlap([torch.zeros(1).expand(5)])
