@@ -558,7 +558,7 @@ int     srwm_b200_rms_forward(const srwm_b200_rms_args* args, void* cuda_stream)
 int     srwm_b200_rms_backward(const srwm_b200_rms_grads* args, void* cuda_stream);
 int64_t srwm_b200_rms_scratch_bytes(int64_t rows, int32_t D);
 
-/* Norm of many tensors (dense, io_dtype each; they must not overlap): *norm = sqrt(sum of squares), and with clip each value times
+/* Norm of many tensors (dense, io_dtype each; with clip they must not overlap): *norm = sqrt(sum of squares), and with clip each value times
  * max_norm / (*norm + 1e-6) where that is below 1 (a NaN among the values goes into all).  `tensors` is read on the host during the
  * call.  scratch of srwm_b200_grads_scratch_bytes, 8-byte aligned. */
 typedef struct srwm_b200_tensor {

@@ -304,7 +304,7 @@ PyObject* grads_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!of_params) ts.push_back(t);
     else if (t.grad().defined()) ts.push_back(t.grad());
   }
-  if (ts.empty() || !grads_ok(ts)) return declined();
+  if (ts.empty() || !grads_ok(ts, max_norm >= 0)) return declined();
   Tensor norm;
   {
     NoGil nogil;

@@ -372,14 +372,14 @@ struct Rms : torch::autograd::Function<Rms> {
 
 // ---- norm over many tensors, clipping ----
 
-// Values of one device that lie dense (in any order) and apart from each other
-inline bool grads_ok(const std::vector<Tensor>& ts) {
+// Values of one device that lie dense (in any order) and, where they are to be written, apart from each other
+inline bool grads_ok(const std::vector<Tensor>& ts, bool written) {
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-  spans.reserve(ts.size());
+  if (written) spans.reserve(ts.size());
   for (const Tensor& t : ts) {
     if (!t.is_cuda() || t.device() != ts[0].device() || !io_ok(t) || t.layout() != at::kStrided || !t.is_non_overlapping_and_dense()) return false;
     const uintptr_t p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-    if (t.numel() > 0) spans.emplace_back(p, p + t.numel() * t.element_size());
+    if (written && t.numel() > 0) spans.emplace_back(p, p + t.numel() * t.element_size());
   }
   std::sort(spans.begin(), spans.end());
   for (size_t i = 1; i < spans.size(); ++i)

@@ -109,7 +109,7 @@ def _checked(tensors, max_norm):
     dense = [t.contiguous() for t in plain]      # (the same memory where it is dense already)
     r = L.host().grads_norm(dense, max_norm, False)
     if r is NotImplemented:
-        raise ValueError("gradients overlap in memory (the same one twice, or views of one another)")
+        raise RuntimeError("these gradients cannot be used")
     if max_norm >= 0.0:
         for t, d in zip(plain, dense):
             if d is not t and d.data_ptr() != t.data_ptr():

@@ -215,3 +215,11 @@ def test_clip_of_views_that_share_values():
     got = sb.grad_ops.clip_tensors_([wide[:, 20:], wide[:, :20:2], wide[:, 1:20:2]], 0.5)
     assert abs(float(got) / float(norm) - 1) < 1e-6
     _near(wide, want[0], 1.5e-6)
+
+
+def test_norm_of_tensors_that_share_values():
+    """Nothing is written: a tensor counts as often as it is there, views and expanded ones among them."""
+    wide = torch.randn(40, 41, device="cuda")
+    for ts in ([wide, wide], [wide, wide[3:9]], [wide[:, 2:30], wide[:, 2:30], wide[:, 3]], [wide[:1].expand(7, -1), wide.to(torch.bfloat16)]):
+        norm, _ = orc.clip(ts, 1.0)
+        assert abs(float(sb.grad_norm(ts)) / float(norm) - 1) < 1e-6
