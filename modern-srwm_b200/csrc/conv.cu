@@ -254,20 +254,22 @@ struct ConvSums {
 __global__ void __launch_bounds__(1024) conv_sums_kernel(const ConvSums a) {
   chained();
   __shared__ float s[32][33];
-  const int c = threadIdx.x % 32, slice = threadIdx.x / 32, total = a.D * (a.K + 1);
-  int i = blockIdx.x * 32 + c;
+  const int c = threadIdx.x % 32, slice = threadIdx.x / 32;
+  const long long total = (long long)a.D * (a.K + 1);
+  long long i = blockIdx.x * 32ll + c;
   float t = 0.f;
   if (i < total) {
 #pragma unroll 8
-    for (int b = slice; b < a.parts; b += 32) t += a.part[(long long)b * total + i];
+    for (int b = slice; b < a.parts; b += 32) t += a.part[b * total + i];
   }
   s[slice][c] = t;
   __syncthreads();
   t = allreduce_warp(s[c][slice]);
-  i = blockIdx.x * 32 + slice;
+  i = blockIdx.x * 32ll + slice;
   if (c != 0 || i >= total) return;
-  const int d = i / (a.K + 1), j = i % (a.K + 1);
-  if (j < a.K) a.dw[(long long)d * a.K + j] = t;
+  const long long d = i / (a.K + 1);
+  const int j = (int)(i - d * (a.K + 1));
+  if (j < a.K) a.dw[d * a.K + j] = t;
   else if (a.dbias) a.dbias[d] = t;
 }
 
@@ -306,7 +308,7 @@ cudaError_t bwd(ConvParams p, cudaStream_t s) {
   if (p.done) conv_bwd_kernel<T, VEC, K, true><<<grid, 128, 0, s>>>(p);
   else conv_bwd_kernel<T, VEC, K, false><<<grid, 128, 0, s>>>(p);
   if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-  return launch_behind(conv_sums_kernel, ConvSums{p.part, p.dw, p.dbias, parts, p.D, K}, dim3((unsigned)((p.D * (K + 1) + 31) / 32)), 1024, 0, s);
+  return launch_behind(conv_sums_kernel, ConvSums{p.part, p.dw, p.dbias, parts, p.D, K}, dim3((unsigned)((p.D * (K + 1ll) + 31) / 32)), 1024, 0, s);
 }
 // f(element, VEC, K)
 template <typename F>

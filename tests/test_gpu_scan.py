@@ -514,3 +514,22 @@ def test_scan_growth_that_a_float_does_not_hold_over_a_piece(S):
         _near(*grads[k], 3e-4, k)
     _near(grads["u"][0][:, 700:800], grads["u"][1][:, 700:800], 3e-4, "in front of the growth")
     assert 1e11 < float(grads["u"][1][:, 500:].abs().max()) < 1e16
+
+
+def test_conv_of_more_than_2_31_weights_and_biases():
+    """The sums of dw and dbias, D (K + 1) values, beyond 32 bits: one step of one sequence, every value a product."""
+    D, K = 860_000_004, 4
+    if torch.cuda.get_device_properties(0).total_memory < 100e9:
+        pytest.skip("100 GB of memory")
+    torch.cuda.empty_cache()
+    x, w = torch.empty(1, 1, D, device="cuda", dtype=torch.bfloat16).normal_().requires_grad_(), torch.full((D, K), 0.5, device="cuda").requires_grad_()
+    bias, gy = torch.zeros(D, device="cuda").requires_grad_(), torch.empty(1, 1, D, device="cuda", dtype=torch.bfloat16).normal_()
+    y, _ = sb.causal_conv(x, w, bias, silu=False)
+    dx, dw, db = torch.autograd.grad(y, [x, w, bias], gy)
+    for a in (0, D // 2, D - 1000):
+        at = slice(a, a + 1000)
+        g, v = gy[0, 0, at].float(), x[0, 0, at].detach().float()
+        assert torch.equal(y[0, 0, at].detach(), (0.5 * v).bfloat16()) and torch.equal(dx[0, 0, at], (0.5 * g).bfloat16())
+        assert torch.equal(db[at], g) and torch.equal(dw[at, K - 1], g * v) and not bool(dw[at, :K - 1].any())
+    del x, w, bias, gy, y, dx, dw, db
+    torch.cuda.empty_cache()
