@@ -931,8 +931,9 @@ static srwm::ScanRows scan_rows(const srwm_b200_seq& t, int X, int es, int* vec)
 }
 static bool off(const void* p, int es) { return (uintptr_t)p % es != 0; }
 
+constexpr int64_t MOST_CHANNELS = 0x3fffffff;      // (twice as many, and a block's more, are still counted in 32 bits)
 static int scan_sizes(int64_t N, int64_t L, int64_t D, int64_t S, int64_t G) {
-  if (N < 0 || L < 0 || D < 0 || G <= 0 || D % G || L > 0x3fff0000LL) return SRWM_B200_ERR_SHAPE;      // (rows behind L are counted too)
+  if (N < 0 || L < 0 || D < 0 || D > MOST_CHANNELS || G <= 0 || D % G || L > 0x3fff0000LL) return SRWM_B200_ERR_SHAPE;      // (rows behind L are counted too)
   if (!head_dim_ok((int)S)) return SRWM_B200_ERR_HEAD_DIM;
   const int64_t blocks = (D / G + 31) / 32 * G;
   // one CTA per sequence and 32 channels; four values of dB or dC per thread of the sums' kernel
@@ -1033,7 +1034,7 @@ extern "C" int srwm_b200_scan_backward(const srwm_b200_scan_args* a, const srwm_
 
 static int conv_params(const srwm_b200_conv_args* a, srwm::ConvParams* p) {
   if (!a) return SRWM_B200_ERR_NULL;
-  if (a->N < 0 || a->L < 0 || a->D < 0 || a->K < 2 || a->K > 4 || a->L > 0x3fff0000) return SRWM_B200_ERR_SHAPE;
+  if (a->N < 0 || a->L < 0 || a->D < 0 || a->D > MOST_CHANNELS || a->K < 2 || a->K > 4 || a->L > 0x3fff0000) return SRWM_B200_ERR_SHAPE;
   if (a->io_dtype != SRWM_B200_F32 && a->io_dtype != SRWM_B200_BF16) return SRWM_B200_ERR_DTYPE;
   const int64_t chunks = a->L == 0 ? 1 : (a->L + srwm::CONV_CHUNK - 1) / srwm::CONV_CHUNK;
   if ((a->D + 3ll) / 4 * chunks / 128 * a->N > 0x7f000000LL) return SRWM_B200_ERR_SHAPE;
@@ -1056,7 +1057,7 @@ static int conv_params(const srwm_b200_conv_args* a, srwm::ConvParams* p) {
   return 0;
 }
 extern "C" int64_t srwm_b200_conv_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t K) {
-  if (N <= 0 || L <= 0 || D <= 0 || K < 2 || K > 4) return 0;
+  if (N <= 0 || L <= 0 || D <= 0 || D > MOST_CHANNELS || K < 2 || K > 4) return 0;
   srwm::ConvParams p = {};
   p.N = N; p.L = L; p.D = D; p.K = K;
   return 4ll * srwm::conv_parts(p) * D * (K + 1);

@@ -197,3 +197,13 @@ def test_gradients_that_share_values():
     assert not _overlap([wide[:, :20], wide[:, 20:], torch.zeros(0)]) and not _overlap([wide[:, ::2], wide[:, 1::2]]) and not _overlap([wide[3:5].t(), wide[5:]])
     assert _overlap([wide[:, :20], wide[:, 19:]]) and _overlap([wide[:, ::2], wide[:, ::2]]) and _overlap([wide[:, 3], wide])
     assert _overlap([torch.zeros(1).expand(5)])
+
+
+@pytest.mark.parametrize("D", [1 << 30, (1 << 31) - 1])
+def test_channels_whose_blocks_are_not_counted_in_32_bits(D):
+    lib = L.load()
+    assert lib.srwm_b200_scan_forward(C.byref(_scan_args(N=1, L=1, D=D)), None) == L.ERR_SHAPE
+    assert lib.srwm_b200_scan_scratch_bytes(1, 1, D, 16, 1) == 0 and lib.srwm_b200_scan_backward_scratch_bytes(1, 1, D, 16, 1) == 0
+    assert lib.srwm_b200_conv_forward(C.byref(_conv_args(N=1, L=1, D=D)), None) == L.ERR_SHAPE
+    assert lib.srwm_b200_conv_backward(C.byref(_conv_args(N=1, L=1, D=D)), C.byref(L.ConvGrads()), None) == L.ERR_SHAPE
+    assert lib.srwm_b200_conv_scratch_bytes(1, 1, D, 4) == 0
