@@ -1,9 +1,11 @@
 // Selective scan, causal convolution, root-mean-square norm and clipping by the gradients' norm, with autograd.
 #pragma once
 #include <algorithm>
+#include <unordered_set>
 #include <vector>
 
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include "host_common.h"
@@ -62,16 +64,34 @@ inline bool rows_apart(const Tensor& t) {
 }
 // A leaf's gradient is gathered on the stream on which a graph first used the leaf.  Where that graph still lives and the stream is
 // the default one, a backward pass under capture would draw the default stream into the capture, which ends the process; said
-// here instead, while the forward pass is captured.
+// here instead, while the forward pass is captured.  The leaves are those of the call and those that this capture has made its
+// arguments of (casts, projections).
 inline void check_capture(std::initializer_list<const Tensor*> ts) {
+  using torch::autograd::Node;
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-  for (const Tensor* t : ts) {
-    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto sum = torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto stream = sum ? sum->stream() : std::nullopt;
-    TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(t->device().index()).unwrap(),
+  auto refuse = [](Node& gathers) {
+    const auto stream = gathers.stream();
+    TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap(),
                 "a leaf of this call belongs to an autograd graph that was built on the default stream and is still alive: drop its "
                 "outputs (a loss, a carried state) before a training step is captured");
+  };
+  std::vector<Node*> open;
+  std::unordered_set<Node*> seen;
+  auto reach = [&](Node* n) {
+    if (n && seen.insert(n).second) open.push_back(n);
+  };
+  for (const Tensor* t : ts) {
+    if (!t->defined() || !t->requires_grad()) continue;
+    if (!t->is_leaf()) reach(t->grad_fn().get());
+    else if (const auto sum = torch::autograd::impl::try_get_grad_accumulator(*t)) refuse(*sum);
+  }
+  while (!open.empty()) {
+    Node* n = open.back();
+    open.pop_back();
+    const auto stream = n->stream();
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(n)) refuse(*n);
+    else if (!stream || *stream == c10::cuda::getCurrentCUDAStream(stream->device_index()).unwrap())
+      for (const auto& e : n->next_edges()) reach(e.function.get());      // (what was there before the capture is not its business)
   }
 }
 

@@ -288,3 +288,35 @@ def test_calls_without_values_have_gradients(N, L, dtype):
     out, st = layer(h, layer.init_state(N), torch.zeros(L, N, dtype=torch.bool, device="cuda"), get_state=True, residual=h)
     assert out.shape == (L, N, 32) and st[0].shape == (N, 3, 64) and st[1].shape == (N, 64, 16)
     assert not any(bool(g.any()) for g in torch.autograd.grad(out.sum(), [h, *layer.parameters()]))
+
+
+def test_capture_of_a_layer_beside_a_living_graph_is_refused():
+    """The same where the operators see casts and products of the leaves, not the leaves themselves; a graph that another stream has
+    built is no obstacle."""
+    layer = _layer(64, 11).to(torch.bfloat16)
+    h = torch.randn(9, 2, 64, device="cuda", dtype=torch.bfloat16)
+    params = list(layer.parameters())
+    go = torch.randn_like(h)
+    alive = layer(h)
+    want = torch.autograd.grad(alive, params, go, retain_graph=True)
+    weight = torch.randn(64, 64, device="cuda", requires_grad=True)
+    other = (weight * 2).sum()
+    for call in (lambda: layer(h), lambda: sb.rms_norm(torch.nn.functional.linear(h.float(), weight), torch.ones(64, device="cuda"))):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match="still alive"):
+                call()
+            keep = h * 2      # (a graph is not empty)
+    del alive, other, graph, keep, call
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = layer(h)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(layer(h), params, go)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph()):
+        layer(h)
