@@ -112,8 +112,8 @@ inline bool scan_ok(const ScanIn& s) {
   const int64_t S = s.A.size(1);
   if (!dense_f32(s.A, {D, S}) || s.A.device() != u.device()) return false;
   for (const Tensor* t : {&s.B, &s.C}) {
-    if (t->device() != u.device() || t->scalar_type() != u.scalar_type() || t->sizes() != s.B.sizes() || !bc_ok(*t)) return false;
-    if ((t->dim() != 3 && t->dim() != 4) || t->size(0) != N || t->size(1) != L || t->size(-1) != S) return false;
+    if (t->device() != u.device() || t->scalar_type() != u.scalar_type() || (t->dim() != 3 && t->dim() != 4)) return false;
+    if (t->sizes() != s.B.sizes() || t->size(0) != N || t->size(1) != L || t->size(-1) != S || !bc_ok(*t)) return false;
     if (t->dim() == 4 && (t->size(2) == 0 || D % t->size(2))) return false;
   }
   for (const Tensor* t : {&s.D, &s.bias})

@@ -533,3 +533,11 @@ def test_conv_of_more_than_2_31_weights_and_biases():
         assert torch.equal(db[at], g) and torch.equal(dw[at, K - 1], g * v) and not bool(dw[at, :K - 1].any())
     del x, w, bias, gy, y, dx, dw, db
     torch.cuda.empty_cache()
+
+
+def test_scan_refuses_b_and_c_of_other_dimensions():
+    x, _, _, _ = _inputs(2, 6, 32, 16, 1, torch.float32)
+    for k in ("B", "C"):
+        for t in (torch.ones((), device="cuda"), torch.ones(16, device="cuda"), torch.ones(2, 6, 1, 1, 16, device="cuda"), torch.ones(2, 6, device="cuda")):
+            with pytest.raises(ValueError):
+                sb.selective_scan(**{**x, k: t})
