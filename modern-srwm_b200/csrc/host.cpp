@@ -45,6 +45,16 @@ bool arity(Py_ssize_t got, Py_ssize_t want) {
   PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
   return false;
 }
+// A truth value; where it has none (a tensor of several values) Python's error goes out.
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) {
+    python_error e;
+    e.persist();
+    throw e;
+  }
+  return v != 0;
+}
 struct NoGil {
   PyThreadState* s = PyEval_SaveThread();
   ~NoGil() { PyEval_RestoreThread(s); }
@@ -228,8 +238,8 @@ PyObject* scan_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!arity(n, 12)) return nullptr;
   Tensor t[10];
   if (forward_ad() || !take(args, 0, 5, t) || !take(args, 5, 5, t + 5, true)) return declined();
-  const ScanIn s = {t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], PyObject_IsTrue(args[10]) != 0};
-  const bool inplace = PyObject_IsTrue(args[11]);
+  const ScanIn s = {t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], truth(args[10])};
+  const bool inplace = truth(args[11]);
   const bool grad = wants_grad({&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8]});
   if (!scan_ok(s) || (inplace && (grad || !s.state.defined()))) return declined();
   if (grad) check_capture({&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8]});
@@ -249,8 +259,8 @@ PyObject* conv_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!arity(n, 7)) return nullptr;
   Tensor t[5];
   if (forward_ad() || !take(args, 0, 2, t) || !take(args, 2, 3, t + 2, true)) return declined();
-  const ConvIn s = {t[0], t[1], t[2], t[3], t[4], PyObject_IsTrue(args[5]) != 0};
-  const bool inplace = PyObject_IsTrue(args[6]), grad = wants_grad({&t[0], &t[1], &t[2], &t[3]});
+  const ConvIn s = {t[0], t[1], t[2], t[3], t[4], truth(args[5])};
+  const bool inplace = truth(args[6]), grad = wants_grad({&t[0], &t[1], &t[2], &t[3]});
   if (!conv_ok(s) || (inplace && (grad || !s.state.defined() || !rows_apart(s.state)))) return declined();
   if (grad) check_capture({&t[0], &t[1], &t[2], &t[3]});
   variable_list r;
@@ -270,7 +280,7 @@ PyObject* rms_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Tensor t[2], res;
   const double eps = PyFloat_AsDouble(args[3]);
   if (eps == -1.0 && PyErr_Occurred()) return nullptr;
-  const bool fp8 = PyObject_IsTrue(args[4]);
+  const bool fp8 = truth(args[4]);
   if (forward_ad() || !take(args, 0, 2, t) || !take(args, 2, 1, &res, true) || !rms_ok(t[0], t[1], res)) return declined();
   const bool grad = wants_grad({&t[0], &t[1], &res});
   if (grad && fp8) return declined();
@@ -290,7 +300,7 @@ PyObject* rms_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* grads_py(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arity(n, 3)) return nullptr;
-  const bool of_params = PyObject_IsTrue(args[2]);
+  const bool of_params = truth(args[2]);
   const double max_norm = PyFloat_AsDouble(args[1]);
   if (max_norm == -1.0 && PyErr_Occurred()) return nullptr;
   if (!PyList_Check(args[0])) return declined();

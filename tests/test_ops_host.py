@@ -207,3 +207,12 @@ def test_channels_whose_blocks_are_not_counted_in_32_bits(D):
     assert lib.srwm_b200_conv_forward(C.byref(_conv_args(N=1, L=1, D=D)), None) == L.ERR_SHAPE
     assert lib.srwm_b200_conv_backward(C.byref(_conv_args(N=1, L=1, D=D)), C.byref(L.ConvGrads()), None) == L.ERR_SHAPE
     assert lib.srwm_b200_conv_scratch_bytes(1, 1, D, 4) == 0
+
+
+def test_options_without_a_truth_value():
+    x, several = torch.zeros(1, 2, 4), torch.ones(2)
+    for call in (lambda: sb.selective_scan(x, x, torch.zeros(4, 8), x, x, delta_softplus=several), lambda: sb.causal_conv(x, torch.zeros(4, 3), silu=several),
+                 lambda: sb.selective_scan(x, x, torch.zeros(4, 8), x, x, inplace_state=several),
+                 lambda: sb.causal_conv(x, torch.zeros(4, 3), inplace_state=several)):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            call()
