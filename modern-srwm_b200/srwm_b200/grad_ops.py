@@ -40,9 +40,9 @@ def clip_tensors_(grads, max_norm, error_if_nonfinite=False):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    grads = list(grads)
     if not grads:
         return torch.zeros(())
-    grads = list(grads)
     if error_if_nonfinite and not torch.isfinite(norm := grad_norm(grads)):
         raise RuntimeError(f"the norm of the gradients is not finite ({float(norm)}); they have not been scaled")
     r = L.host().grads_norm(grads, max_norm, False)

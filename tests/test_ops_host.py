@@ -216,3 +216,8 @@ def test_options_without_a_truth_value():
                  lambda: sb.causal_conv(x, torch.zeros(4, 3), inplace_state=several)):
         with pytest.raises(RuntimeError, match="ambiguous"):
             call()
+
+
+def test_clipping_an_iterator_that_is_empty():
+    assert float(sb.grad_ops.clip_tensors_(iter(()), 1.0)) == 0.0 and float(sb.grad_norm(iter(()))) == 0.0
+    assert float(sb.clip_grad_norm_(iter(()), 1.0)) == 0.0
