@@ -73,6 +73,8 @@ class GradBucket:
         if self.flat.device.type == "cuda":
             from .grad_ops import clip_tensors_
             return clip_tensors_([self.flat], max_norm)
+        if not max_norm >= 0.0:
+            raise ValueError(f"max_norm must not be negative, got {max_norm}")
         norm = self.flat.norm()
         self.flat.mul_(torch.clamp(max_norm / (norm + 1e-6), max=1.0))
         return norm

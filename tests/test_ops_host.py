@@ -221,3 +221,12 @@ def test_options_without_a_truth_value():
 def test_clipping_an_iterator_that_is_empty():
     assert float(sb.grad_ops.clip_tensors_(iter(()), 1.0)) == 0.0 and float(sb.grad_norm(iter(()))) == 0.0
     assert float(sb.clip_grad_norm_(iter(()), 1.0)) == 0.0
+
+
+def test_bucket_refuses_a_negative_norm_on_the_cpu():
+    b = GradBucket([(4,)], "cpu")
+    b.view(0).fill_(3.0)
+    for most in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            b.clip_(most)
+    assert bool((b.flat == 3.0).all())
