@@ -541,3 +541,33 @@ def test_scan_refuses_b_and_c_of_other_dimensions():
         for t in (torch.ones((), device="cuda"), torch.ones(16, device="cuda"), torch.ones(2, 6, 1, 1, 16, device="cuda"), torch.ones(2, 6, device="cuda")):
             with pytest.raises(ValueError):
                 sb.selective_scan(**{**x, k: t})
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("K", [2, 3, 4])
+@pytest.mark.parametrize("L,reset", [(9, 4), (100, 16), (100, 33), (300, 150)])
+def test_conv_bad_values_do_not_pass_a_reset(L, reset, K, bad):
+    """Inputs, states and gradients of one episode that are NaN or infinite leave every bit of the other's, at the edges of the chunks of
+    the time axis too."""
+    g = torch.Generator(device="cuda").manual_seed(L + K)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    x, w, b, st, gy, gs = r(2, L, 40), r(40, K), r(40), r(2, K - 1, 40), r(2, L, 40), r(2, K - 1, 40)
+    done = torch.zeros(2, L, dtype=torch.bool, device="cuda")
+    done[0, reset] = True
+
+    def both(x, st, gy):
+        args = [t.detach().requires_grad_() for t in (x, st)]
+        y, s = sb.causal_conv(args[0], w, b, args[1], done)
+        return [y.detach(), s.detach(), *torch.autograd.grad([y, s], args, [gy, gs])]
+    y, s, dx, ds = both(x, st, gy)
+    for at in range(max(0, reset - K), reset):
+        spoilt, recycled = x.clone(), st.clone()
+        spoilt[0, at], recycled[0] = bad, bad
+        got = both(spoilt, recycled, gy)
+        assert torch.equal(got[0][0, reset:], y[0, reset:]) and torch.equal(got[1], s) and torch.equal(got[2][0, reset:], dx[0, reset:])
+        assert torch.equal(got[0][1], y[1]) and torch.equal(got[2][1], dx[1]) and not bool(torch.isfinite(got[0][0, at]).any())
+    for at in range(reset, min(L, reset + K)):
+        gy_bad, spoilt = gy.clone(), x.clone()
+        gy_bad[0, at], spoilt[0, at] = bad, bad
+        got = both(spoilt, st, gy_bad)
+        assert torch.equal(got[0][0, :reset], y[0, :reset]) and torch.equal(got[2][0, :reset], dx[0, :reset]) and torch.equal(got[3], ds)
