@@ -456,7 +456,7 @@ int srwm_b200_block_forward(const srwm_b200_block_args* args, void* cuda_stream)
  * for each of D channels with S states.  Rows are [N, L, X] views, innermost contiguous, any other strides (elements), starting
  * on their elements' alignment; rows whose pieces of four elements are aligned are read four at a time.  B and C are [N, L, G, S]: channel
  * d reads group d / (D / G).  A [D, S], D, delta_bias [D], states [N, D, S]: dense fp32; A and the states on 16-byte boundaries.
- * S is 8, 16, 32 or 64 (otherwise ERR_HEAD_DIM); D is a multiple of G.  done [N, L] (bytes, any strides) not zero: the state in
+ * S is 8, 16, 32 or 64 (otherwise ERR_HEAD_DIM); D is a multiple of G, below 2^30.  done [N, L] (bytes, any strides) not zero: the state in
  * front of step t is zero.  state_out may be state_in.  L == 0 copies the state.
  * `checkpoints` [N, ceil(L / 8), D, S] (srwm_b200_scan_checkpoint_floats), 16-byte aligned, is written for the backward (NULL: no
  * backward).  `scratch` (srwm_b200_scan_scratch_bytes / _backward_scratch_bytes, 0: may be NULL) is used during the call.
@@ -499,7 +499,7 @@ int64_t srwm_b200_scan_checkpoint_floats(int32_t N, int32_t L, int32_t D, int32_
 int64_t srwm_b200_scan_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S, int32_t G);
 int64_t srwm_b200_scan_backward_scratch_bytes(int32_t N, int32_t L, int32_t D, int32_t S, int32_t G);
 
-/* y_t = act(bias + sum_i w[K-1-i] x_{t-i}), act = silu or the identity, K = 2, 3 or 4 taps (otherwise ERR_SHAPE); w [D, K], bias [D] dense
+/* y_t = act(bias + sum_i w[K-1-i] x_{t-i}), act = silu or the identity, K = 2, 3 or 4 taps (otherwise ERR_SHAPE), D below 2^30; w [D, K], bias [D] dense
  * fp32.  state_in / state_out [N, K-1, D] in the rows' type: the last K - 1 inputs before the call and at its end (NULL: zeros / not
  * wanted); state_out may be state_in where L <= 16.  done as above: no input in front of an episode's start is read behind it.
  * Backward: dstate_out NULL: zeros; dstate_in, dbias NULL: not wanted; scratch of srwm_b200_conv_scratch_bytes. */

@@ -4,8 +4,10 @@
 //
 // Bound by HBM: one read and one write of [N, L, D].  A thread takes four channels and a chunk of steps in time order, its window in
 // registers, the next steps' rows on their way; the K - 1 steps in front of its own come from L2.  8 x 2048 x 2048, K 4, bf16: forward 32 us
-// (21 at the copy bandwidth), backward 57 (31).  Chunks as long as fill the GPU once, and steps inside a chunk without conditions, took
-// them there from 39 and 75 with chunks of 16: the backward's instructions bind, a hundred for four channels and a step.
+// (21 at the copy bandwidth), backward 57 (31: x is read again).  Chunks as long as fill the GPU once, and steps inside a chunk without
+// conditions, took them there from 39 and 75 with chunks of 16.  Both wait for memory: issue is busy 41 % of the time, the loads are the first
+// stall, and the backward's three blocks of 144 registers a thread have 24 KB of rows on their way a multiprocessor, where the copy
+// bandwidth times its latency is some 35.  (Some variants keep a value or two of a thread on the stack, 4 to 48 bytes.)
 #include <type_traits>
 
 #include "chain.h"

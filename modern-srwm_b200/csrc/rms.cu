@@ -3,7 +3,7 @@
 // y in the type of x, or in e4m3 with one scale a row: scale = max |y| / 448 (at least 2^-126), y / scale rounded to nearest.
 //
 // Bound by HBM: x and res in, s and y out, once each (16384 x 512 fp32 with the residual: forward 19 us, backward 20 + 4, 20.5 each
-// at the copy bandwidth; loads behind branches instead of predicates took 29 and 55).  A row stays in registers between its sum and its result: up to 1024 columns with a
+// at the copy bandwidth, which L2 has part of in passes one after another; loads behind branches instead of predicates took 29 and 55).  A row stays in registers between its sum and its result: up to 1024 columns with a
 // warp, above with a block of eight warps.  The weight's gradient is kept per thread over all rows of a block and added up over
 // the blocks by a second launch, in a fixed order.
 #include "rms.h"

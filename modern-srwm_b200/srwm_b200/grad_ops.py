@@ -1,10 +1,10 @@
-"""Global gradient norm over many tensors, and clipping by it, in two launches however many tensors there are.
+"""Global gradient norm over many tensors, and clipping by it, in two launches for each 1024 of them.
 
     clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False) -> norm
         the gradients of the parameters times max_norm / (norm + 1e-6) where that is below 1, in place, norm their 2-norm before;
         the same values as torch.nn.utils.clip_grad_norm_ (a NaN among them makes all of them NaN)
     grad_norm(tensors) -> norm
-        the 2-norm over all values of a list of tensors
+        the 2-norm over all values of a list of tensors (which may share memory; gradients that are clipped may not)
 
 float32 and bfloat16 tensors of one device, mixed; the sum is fp32 over 32 values and fp64 from there on, in a fixed order.  The norm
 stays on the device (a 0-dimensional float32 tensor): nothing waits for it.  With several ranks the gradients are all-reduced
