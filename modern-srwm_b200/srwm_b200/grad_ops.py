@@ -51,6 +51,8 @@ def clip_tensors_(grads, max_norm, error_if_nonfinite=False):
 
 def _bytes(t):
     """[(distance, count)] of a tensor's bytes, the largest distance first."""
+    if t.is_contiguous():
+        return [(1, t.numel() * t.element_size())]
     dims = [(st * t.element_size(), n) for st, n in zip(t.stride(), t.shape) if n > 1] + [(1, t.element_size())]
     return sorted(dims, reverse=True)
 
