@@ -62,39 +62,6 @@ inline bool rows_apart(const Tensor& t) {
   const int a = t.stride(0) >= t.stride(1) ? 0 : 1, b = 1 - a;      // the rows further apart, and the others
   return (t.size(b) == 1 || t.stride(b) >= t.size(2)) && (t.size(a) == 1 || t.stride(a) >= (t.size(b) == 1 ? 0 : t.stride(b) * (t.size(b) - 1)) + t.size(2));
 }
-// A leaf's gradient is gathered on the stream on which a graph first used the leaf.  Where that graph still lives and the stream is
-// the default one, a backward pass under capture would draw the default stream into the capture, which ends the process; said
-// here instead, while the forward pass is captured.  The leaves are those of the call and those that this capture has made its
-// arguments of (casts, projections).
-inline void check_capture(std::initializer_list<const Tensor*> ts) {
-  using torch::autograd::Node;
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-  auto refuse = [](Node& gathers) {
-    const auto stream = gathers.stream();
-    TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap(),
-                "a leaf of this call belongs to an autograd graph that was built on the default stream and is still alive: drop its "
-                "outputs (a loss, a carried state) before a training step is captured");
-  };
-  std::vector<Node*> open;
-  std::unordered_set<Node*> seen;
-  auto reach = [&](Node* n) {
-    if (n && seen.insert(n).second) open.push_back(n);
-  };
-  for (const Tensor* t : ts) {
-    if (!t->defined() || !t->requires_grad()) continue;
-    if (!t->is_leaf()) reach(t->grad_fn().get());
-    else if (const auto sum = torch::autograd::impl::try_get_grad_accumulator(*t)) refuse(*sum);
-  }
-  while (!open.empty()) {
-    Node* n = open.back();
-    open.pop_back();
-    const auto stream = n->stream();
-    if (dynamic_cast<torch::autograd::AccumulateGrad*>(n)) refuse(*n);
-    else if (!stream || *stream == c10::cuda::getCurrentCUDAStream(stream->device_index()).unwrap())
-      for (const auto& e : n->next_edges()) reach(e.function.get());      // (what was there before the capture is not its business)
-  }
-}
-
 // ---- selective scan ----
 
 struct ScanIn {
@@ -389,6 +356,44 @@ struct Rms : torch::autograd::Function<Rms> {
     return {dx, dw, has_res ? dx : Tensor(), Tensor()};
   }
 };
+
+// ---- captures ----
+
+// A leaf's gradient is gathered on the stream on which a graph first used the leaf.  Where that graph still lives and the stream is
+// the default one, a backward pass under capture would draw the default stream into the capture, which ends the process; said
+// here instead, while the forward pass is captured.  The leaves are those of the call and those that this capture has made its
+// arguments of (casts, projections), up to operators of this file, which have asked already.
+inline void check_capture(std::initializer_list<const Tensor*> ts) {
+  using torch::autograd::Node;
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  auto refuse = [](Node& gathers) {
+    const auto stream = gathers.stream();
+    TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap(),
+                "a leaf of this call belongs to an autograd graph that was built on the default stream and is still alive: drop its "
+                "outputs (a loss, a carried state) before a training step is captured");
+  };
+  std::vector<Node*> open;
+  std::unordered_set<Node*> seen;
+  auto reach = [&](Node* n) {
+    if (n && seen.insert(n).second) open.push_back(n);
+  };
+  for (const Tensor* t : ts) {
+    if (!t->defined() || !t->requires_grad()) continue;
+    if (!t->is_leaf()) reach(t->grad_fn().get());
+    else if (const auto sum = torch::autograd::impl::try_get_grad_accumulator(*t)) refuse(*sum);
+  }
+  while (!open.empty()) {
+    Node* n = open.back();
+    open.pop_back();
+    if (dynamic_cast<torch::autograd::CppNode<Scan>*>(n) || dynamic_cast<torch::autograd::CppNode<Conv>*>(n) ||
+        dynamic_cast<torch::autograd::CppNode<Rms>*>(n))
+      continue;
+    const auto stream = n->stream();
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(n)) refuse(*n);
+    else if (!stream || *stream == c10::cuda::getCurrentCUDAStream(stream->device_index()).unwrap())
+      for (const auto& e : n->next_edges()) reach(e.function.get());      // (what was there before the capture is not its business)
+  }
+}
 
 // ---- norm over many tensors, clipping ----
 
