@@ -458,6 +458,7 @@ int srwm_b200_block_forward(const srwm_b200_block_args* args, void* cuda_stream)
  * d reads group d / (D / G).  A [D, S], D, delta_bias [D], states [N, D, S]: dense fp32; A and the states on 16-byte boundaries.
  * S is 8, 16, 32 or 64 (otherwise ERR_HEAD_DIM); D is a multiple of G, below 2^30.  done [N, L] (bytes, any strides) not zero: the state in
  * front of step t is zero.  state_out may be state_in.  L == 0 copies the state.
+ * Here and in the next two sections a call of no sequences, channels or rows succeeds and writes nothing, the parameters' gradients neither.
  * `checkpoints` [N, ceil(L / 8), D, S] (srwm_b200_scan_checkpoint_floats), 16-byte aligned, is written for the backward (NULL: no
  * backward).  `scratch` (srwm_b200_scan_scratch_bytes / _backward_scratch_bytes, 0: may be NULL) is used during the call.
  * ---------------------------------------------------------------------------------- */
